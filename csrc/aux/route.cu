@@ -1,0 +1,406 @@
+// Routing of tokens to experts: scores of the router's logits, choice of the k experts of a token, their weights, and
+// the gradient of the weights with respect to the logits.
+//
+//   s = softmax(l) over the E experts, or sigmoid(l) of each          c = s + bias  (the bias steers the choice only)
+//   G groups of E / G consecutive experts: a group's score is the sum of its `group_top` largest c; the `topk_groups`
+//   best groups stay. Of their experts the k with the largest c are chosen, largest first.
+//   w = scale * s[chosen] / sum(s[chosen])   (renormalised), or scale * s[chosen]
+// Equal values go to the lower index, NaN counts as the lowest value there is. A row that masks every expert (all -inf)
+// gets the lowest indices with weights of zero: the k indices of a token are always valid and different.
+//
+// Backward, with g = dL/dw and D = sum_j g_j w_j:
+//   sigmoid, renormalised    dl_i = w_i (g_i - D / scale) (1 - s_i)      sigmoid, plain   dl_i = w_i g_i (1 - s_i)
+//   softmax, renormalised    dl_i = w_i (g_i - D / scale)                softmax, plain   dl_e = [e chosen] w_e g_e - p_e D
+// (the renormalised softmax is the softmax over the chosen experts alone, which is why p drops out).
+//
+// One warp per token; a lane holds PER consecutive experts, so that the lowest lane with the largest value holds the
+// lowest index, and a row is read in 16-byte pieces.
+#include "../include/fluxb.h"
+#include "../runtime/host_common.h"
+#include "../sm100/ptx.cuh"
+
+#include <atomic>
+
+namespace fluxb {
+extern std::atomic<uint64_t> g_launches;
+
+namespace {
+
+constexpr int kRouteWarps = 4;
+constexpr int kRouteMaxExperts = 512;
+constexpr int kRouteMaxGroups = 32;
+constexpr unsigned kFull = 0xffffffffu;
+
+struct RouteParams {
+  const void* logits;
+  int64_t row_stride;            // elements
+  const float* bias;             // [E] or null
+  int32_t* experts;              // [tokens, k]
+  float* weights;                // [tokens, k]
+  const float* grad;             // backward: [tokens, k]
+  void* dlogits;                 // backward: [tokens, E], type of the logits
+  int64_t tokens;
+  int32_t E, k, groups, topk_groups, group_top, sigmoid, renorm, vec;
+  float scale;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// Unsigned keys in the order of the values. 0: no candidate, 1: NaN, then -inf and up; both zeros have one key.
+__device__ __forceinline__ uint64_t key_of(double v) {
+  if (isnan(v)) return 1ull;
+  const int64_t b = __double_as_longlong(v + 0.0);
+  return static_cast<uint64_t>(b) ^ (static_cast<uint64_t>(b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double value_of(uint64_t key) {
+  const uint64_t b = key >> 63 ? key ^ 0x8000000000000000ull : ~key;
+  return __longlong_as_double(static_cast<int64_t>(b));
+}
+// largest key of the warp
+__device__ __forceinline__ uint64_t warp_max(uint64_t key) {
+  const uint32_t hi = static_cast<uint32_t>(key >> 32);
+  const uint32_t top = __reduce_max_sync(kFull, hi);
+  const uint32_t low = __reduce_max_sync(kFull, hi == top ? static_cast<uint32_t>(key) : 0u);
+  return static_cast<uint64_t>(top) << 32 | low;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+// (fmaxf passes NaN over)
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
+// This lane's PER logits of one row; -inf past the last expert.
+template <typename T, int PER>
+__device__ __forceinline__ void load_row(const RouteParams& p, int64_t token, int lane, float (&l)[PER]) {
+  constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
+  const T* row = static_cast<const T*>(p.logits) + token * p.row_stride;
+  const int e0 = lane * PER;
+  if (p.vec) {
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+      struct alignas(sizeof(T) * V) Piece { T v[V]; };
+      Piece piece;
+      const bool in = e0 + i < p.E;            // (E is a multiple of V then)
+      if (in) piece = *reinterpret_cast<const Piece*>(row + e0 + i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) l[i + j] = in ? to_f32(piece.v[j]) : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) l[i] = e0 + i < p.E ? to_f32(row[e0 + i]) : -INFINITY;
+  }
+}
+
+// Takes the largest of the lanes' keys k times; the lane of the winner drops it. Lane j < k returns the j-th expert.
+template <int PER>
+__device__ __forceinline__ int take_best(uint64_t (&key)[PER], int k, int lane) {
+  int mine = 0;
+  for (int j = 0; j < k; ++j) {
+    uint64_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < PER; ++i) {
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    }
+    const uint64_t top = warp_max(best);
+    const int winner = __ffs(__ballot_sync(kFull, best == top)) - 1;
+    const int e = __shfl_sync(kFull, lane * PER + at, winner);
+    if (lane == j) mine = e;
+    if (lane == winner) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i == at) key[i] = 0;
+    }
+  }
+  return mine;
+}
+
+// The choice in 64 bits: scores, group scores and comparisons in double precision. Without a bias the scores have the
+// order of the logits, which are compared as they are (scores that round to the same number stay apart).
+template <int PER>
+__device__ __forceinline__ int choose64(const RouteParams& p, const float (&l)[PER], float row_max, int lane,
+                                        uint64_t* keys /* shared, [E], with groups */) {
+  const int e0 = lane * PER;
+  uint64_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = e0 + i < p.E ? key_of(static_cast<double>(l[i])) : 0ull;
+  if (p.bias != nullptr || (p.groups > 1 && p.group_top == 2)) {
+    double s[PER];
+    if (p.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(l[i])));
+    } else {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        s[i] = row_max == -INFINITY ? (isnan(l[i]) ? NAN : 0.0) : exp(static_cast<double>(l[i]) - static_cast<double>(row_max));
+        sum += s[i];
+      }
+      sum = warp_sum(sum);
+      if (sum != 0.0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s[i] /= sum;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = e0 + i < p.E;
+      if (p.bias != nullptr && in) key[i] = key_of(s[i] + static_cast<double>(p.bias[e0 + i]));
+      if (p.groups > 1 && in) keys[e0 + i] = p.bias != nullptr ? key[i] : key_of(s[i]);
+    }
+  } else if (p.groups > 1) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i < p.E) keys[e0 + i] = key[i];
+  }
+  if (p.groups > 1) {
+    const int size = p.E / p.groups;
+    __syncwarp();
+    uint64_t mine = 0;             // lane g: key of group g's score
+    for (int g = 0; g < p.groups; ++g) {
+      uint64_t a = 0, b = 0;       // the two largest of this lane's share
+      for (int i = lane; i < size; i += 32) {
+        const uint64_t x = keys[g * size + i];
+        if (x > a) {
+          b = a;
+          a = x;
+        } else if (x > b) {
+          b = x;
+        }
+      }
+      const uint64_t first = warp_max(a);
+      uint64_t total = first;
+      if (p.group_top == 2) {
+        const int winner = __ffs(__ballot_sync(kFull, a == first)) - 1;
+        const uint64_t second = warp_max(lane == winner ? b : a);
+        // (key 1 stands for NaN, which makes the sum the lowest too)
+        total = first == 1 || second == 1 ? 1ull : key_of(value_of(first) + value_of(second));
+      }
+      if (lane == g) mine = total;
+    }
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const uint64_t other = __shfl_sync(kFull, mine, g);
+      rank += other > mine || (other == mine && g < lane) ? 1 : 0;
+    }
+    const unsigned kept = __ballot_sync(kFull, lane < p.groups && rank < p.topk_groups);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i < p.E && !(kept >> ((e0 + i) / size) & 1u)) key[i] = 0;
+    __syncwarp();
+  }
+  return take_best<PER>(key, p.k, lane);
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
+  extern __shared__ uint64_t group_keys[];          // [warps][E], with groups only
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
+  if (token >= p.tokens) return;
+  float l[PER];
+  load_row<T, PER>(p, token, lane, l);
+  float top = l[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) top = fmaxf(top, l[i]);
+  const float row_max = warp_max(top);
+  const int e = choose64<PER>(p, l, row_max, lane, group_keys + warp * p.E);
+
+  // weights: lane j holds the j-th expert
+  const bool live = lane < p.k;
+  const float le = live ? to_f32(static_cast<const T*>(p.logits)[token * p.row_stride + e]) : -INFINITY;
+  float w;
+  if (p.sigmoid) {
+    // sigmoid(l) exp(-c) with c the largest chosen logit if that is negative: the quotient keeps its digits where all
+    // the sigmoids are close to zero
+    const float c = p.renorm ? fminf(warp_max(le), 0.f) : 0.f;
+    w = le >= 0.f ? 1.f / (1.f + expf(-le)) : expf(le - c) / (1.f + expf(le));
+    if (live && le == -INFINITY) w = 0.f;
+  } else {
+    // (a NaN in the row reaches every weight, as in any softmax)
+    float sum = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      nan |= isnan(l[i]);
+      sum += p.renorm || row_max == -INFINITY ? 0.f : expf(l[i] - row_max);
+    }
+    if (!p.renorm) sum = warp_sum(sum);
+    if (__any_sync(kFull, nan)) sum = NAN;
+    const float c = p.renorm ? warp_max(le) : row_max;
+    w = c == -INFINITY ? 0.f : expf(le - c);
+    if (isnan(sum)) w = NAN;
+    else if (!p.renorm) w = sum > 0.f ? w / sum : 0.f;
+  }
+  if (p.renorm) {
+    const float total = warp_sum(live ? w : 0.f);
+    w = total == 0.f ? 0.f : w / total;
+  }
+  if (live) {
+    p.experts[token * p.k + lane] = e;
+    p.weights[token * p.k + lane] = w * p.scale;
+  }
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_bwd_kernel(const RouteParams p) {
+  constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
+  if (token >= p.tokens) return;
+  const bool live = lane < p.k;
+  const int e = live ? p.experts[token * p.k + lane] : 0;
+  const float w = live ? p.weights[token * p.k + lane] : 0.f;
+  const float g = live ? p.grad[token * p.k + lane] : 0.f;
+  const float dot = warp_sum(w * g);
+  const T* row = static_cast<const T*>(p.logits) + token * p.row_stride;
+  T* out = static_cast<T*>(p.dlogits) + token * p.E;
+  const int e0 = lane * PER;
+  float d[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) d[i] = 0.f;
+  if (!p.sigmoid && !p.renorm) {
+    float l[PER];
+    load_row<T, PER>(p, token, lane, l);
+    float top = l[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) top = fmaxf(top, l[i]);
+    const float row_max = warp_max(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      d[i] = row_max == -INFINITY ? (isnan(l[i]) ? l[i] : 0.f) : expf(l[i] - row_max);
+      sum += d[i];
+    }
+    sum = warp_sum(sum);
+    const float f = sum == 0.f ? 0.f : -dot / sum;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) d[i] *= f;
+  }
+  // the chosen experts' terms, added where they belong
+  float mine;
+  if (p.renorm) {
+    mine = w * (g - dot / p.scale);
+  } else {
+    mine = w * g;
+  }
+  if (p.sigmoid && live) {
+    const float le = to_f32(row[e]);
+    mine *= le >= 0.f ? expf(-le) / (1.f + expf(-le)) : 1.f / (1.f + expf(le));
+  }
+  for (int j = 0; j < p.k; ++j) {
+    const int ej = __shfl_sync(kFull, e, j);
+    const float v = __shfl_sync(kFull, mine, j);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i == ej) d[i] += v;
+  }
+  if (p.E % V == 0) {
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+      struct alignas(sizeof(T) * V) Piece { T v[V]; };
+      Piece piece;
+#pragma unroll
+      for (int j = 0; j < V; ++j) piece.v[j] = from_f32<T>(d[i + j]);
+      if (e0 + i < p.E) *reinterpret_cast<Piece*>(out + e0 + i) = piece;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i < p.E) out[e0 + i] = from_f32<T>(d[i]);
+  }
+}
+
+template <typename T, int PER>
+int launch_route(RouteParams& p, bool backward, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T) < PER ? 16 / sizeof(T) : PER;
+  p.vec = p.E % V == 0 && p.row_stride % V == 0 && reinterpret_cast<uintptr_t>(p.logits) % (V * sizeof(T)) == 0;
+  const int64_t grid = (p.tokens + kRouteWarps - 1) / kRouteWarps;
+  FLUXB_REQUIRE(grid <= 0x7fffffff, "too many tokens");
+  if (backward) {
+    route_bwd_kernel<T, PER><<<static_cast<unsigned>(grid), kRouteWarps * 32, 0, stream>>>(p);
+  } else {
+    const size_t smem = p.groups > 1 ? sizeof(uint64_t) * kRouteWarps * p.E : 0;
+    route_kernel<T, PER><<<static_cast<unsigned>(grid), kRouteWarps * 32, smem, stream>>>(p);
+  }
+  FLUXB_CUDA_OK(cudaGetLastError());
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return kOk;
+}
+
+template <typename T>
+int launch_route(RouteParams& p, bool backward, cudaStream_t stream) {
+  if (p.E <= 64) return launch_route<T, 2>(p, backward, stream);
+  if (p.E <= 128) return launch_route<T, 4>(p, backward, stream);
+  if (p.E <= 256) return launch_route<T, 8>(p, backward, stream);
+  return launch_route<T, 16>(p, backward, stream);
+}
+
+int route(const fluxb_route_args_t* a, bool backward) {
+  FLUXB_REQUIRE(a != nullptr, "null arguments");
+  FLUXB_REQUIRE(a->tokens >= 0 && a->num_experts >= 1 && a->num_experts <= kRouteMaxExperts, "routing sizes");
+  FLUXB_REQUIRE(a->num_groups >= 1 && a->num_groups <= kRouteMaxGroups && a->num_experts % a->num_groups == 0,
+                "experts must divide over at most 32 groups");
+  const int size = a->num_experts / a->num_groups;
+  FLUXB_REQUIRE(a->topk_groups >= 1 && a->topk_groups <= a->num_groups, "groups to keep");
+  FLUXB_REQUIRE(a->group_top == 1 || (a->group_top == 2 && size >= 2), "group scores sum one or two experts");
+  FLUXB_REQUIRE(a->topk >= 1 && a->topk <= 32 && a->topk <= a->topk_groups * size, "experts per token");
+  if (a->tokens == 0) return kOk;
+  FLUXB_REQUIRE(a->logits && a->experts && a->weights, "null routing tensors");
+  FLUXB_REQUIRE(!backward || (a->grad && a->dlogits), "null gradients");
+  FLUXB_REQUIRE(a->row_stride >= 0, "row stride");
+  FLUXB_REQUIRE(a->scale != 0.f && a->scale - a->scale == 0.f, "scale must be finite and not zero");
+  RouteParams p = {};
+  p.logits = a->logits;
+  p.row_stride = a->row_stride;
+  p.bias = a->bias;
+  p.experts = a->experts;
+  p.weights = a->weights;
+  p.grad = a->grad;
+  p.dlogits = a->dlogits;
+  p.tokens = a->tokens;
+  p.E = a->num_experts;
+  p.k = a->topk;
+  p.groups = a->num_groups;
+  p.topk_groups = a->topk_groups;
+  p.group_top = a->group_top;
+  p.sigmoid = a->score == FLUXB_SCORE_SIGMOID;
+  p.renorm = a->renormalize != 0;
+  p.scale = a->scale;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+  switch (a->dtype) {
+    case FLUXB_FP32: return launch_route<float>(p, backward, stream);
+    case FLUXB_BF16: return launch_route<__nv_bfloat16>(p, backward, stream);
+    case FLUXB_FP16: return launch_route<__half>(p, backward, stream);
+    default: return fail(kErrUnsupported, "routing takes fp32, bf16 or fp16 logits");
+  }
+}
+
+}  // namespace
+}  // namespace fluxb
+
+using namespace fluxb;
+
+extern "C" int fluxb_moe_route(const fluxb_route_args_t* args) { return route(args, false); }
+extern "C" int fluxb_moe_route_bwd(const fluxb_route_args_t* args) { return route(args, true); }

@@ -374,6 +374,81 @@ int fluxb_moe_index_build(const int32_t* experts, int64_t n, int E, int topk, in
                           int32_t* offsets, int32_t* scatter_index, int32_t* gather_index,
                           int32_t* topk_index, int32_t* scratch, void* stream);
 
+/* ---- routing of tokens to experts (see csrc/aux/route.cu for the definition) ---- */
+enum { FLUXB_SCORE_SOFTMAX = 0, FLUXB_SCORE_SIGMOID = 1 };
+typedef struct {
+  const void* logits;        /* [tokens, num_experts], fp32 | bf16 | fp16, rows row_stride elements apart */
+  const float* bias;         /* [num_experts] added to the scores for the choice, or null */
+  int32_t* experts;          /* [tokens, topk]: written by the forward, read by the backward */
+  float* weights;            /* [tokens, topk]: written by the forward, read by the backward */
+  const float* grad;         /* backward: gradient of the weights */
+  void* dlogits;             /* backward: [tokens, num_experts] in the type of the logits */
+  int64_t tokens, row_stride;
+  int32_t num_experts;       /* at most 512 */
+  int32_t topk;              /* at most 32 */
+  int32_t num_groups, topk_groups, group_top;
+  int32_t score;             /* FLUXB_SCORE_* */
+  int32_t renormalize, dtype;
+  float scale;
+  int32_t reserved;
+  void* stream;
+} fluxb_route_args_t;
+int fluxb_moe_route(const fluxb_route_args_t* args);
+int fluxb_moe_route_bwd(const fluxb_route_args_t* args);
+
+/* ---- gated activation y = r * act(gate) * up and its gradient (see csrc/aux/gated.cu) ---- */
+typedef struct {
+  const void* gate;          /* [rows, cols], rows gate_stride elements apart */
+  const void* up;            /* [rows, cols], rows up_stride elements apart */
+  const float* row_weight;   /* [rows] or null: r = 1 */
+  const void* num_rows;      /* device: rows in use (int32, or int64 if num_rows_64); null: all */
+  void* out;                 /* forward: [rows, cols], rows out_stride elements apart */
+  const void* grad;          /* backward: gradient of out, rows grad_stride elements apart */
+  void* dgate;               /* backward, rows dgate_stride elements apart; dup likewise */
+  void* dup;
+  float* drow;               /* backward: [rows] or null */
+  int64_t rows, gate_stride, up_stride, out_stride, grad_stride, dgate_stride, dup_stride;
+  int32_t cols, dtype;       /* bf16 | fp16 | fp32 */
+  int32_t act;               /* 1 gelu(tanh), 2 relu, 3 silu */
+  int32_t num_rows_64;
+  int32_t zero_rest;         /* rows that are not in use: 1 written as zeros, 0 left as they are */
+  int32_t reserved;
+  void* stream;
+} fluxb_gated_args_t;
+int fluxb_gated_act(const fluxb_gated_args_t* args);
+int fluxb_gated_act_bwd(const fluxb_gated_args_t* args);
+
+/* ---- products with 4-bit weights: out[m, n] = sum_k x[m, k] * (q[n, k] - z[n, k / group]) * s[n, k / group] (+ bias[n]),
+ * dense, or for E experts over rows sorted by expert (see csrc/sm100/gemm_int4.cuh for the layouts) ---- */
+typedef struct {
+  const uint8_t* q;          /* [E, N, K / 2]: value 2j in the low half of byte j */
+  const void* scales;        /* [E, N, K / group], bf16 | fp16 */
+  const uint8_t* zeros;      /* [E, N, K / group] in 0 .. 15, or null: 8 */
+  void* packed;              /* [E][Np / 16][Kp / 64][512 bytes], Np and Kp: N and K rounded up to 128; 16-byte aligned */
+  void* scales_out;          /* [E][Kp / min(group, 128)][Np], 16 bits each; 16-byte aligned */
+  uint8_t* zeros_out;        /* the same in bytes; null without zeros */
+  int32_t experts, N, K, group;
+  void* stream;
+} fluxb_int4_layout_t;
+int fluxb_int4_layout(const fluxb_int4_layout_t* args);
+
+typedef struct {
+  const void* x;             /* [M, K], rows ldx elements apart, 16-byte aligned rows */
+  const void* packed;        /* as fluxb_int4_layout leaves them */
+  const void* scales;
+  const uint8_t* zeros;
+  const void* bias;          /* [N] in the type of x, or null */
+  const int32_t* splits;     /* grouped: rows of each expert, on the device; null: dense */
+  void* out;                 /* [M, N], rows ldo elements apart */
+  int64_t M, ldx, ldo;
+  int32_t experts, N, K, group;
+  int32_t dtype;             /* of x and out: bf16 | fp16 */
+  int32_t scale_dtype;       /* bf16 | fp16 */
+  fluxb_status_t* status;    /* device memory, may be null */
+  void* stream;
+} fluxb_int4_gemm_t;
+int fluxb_int4_gemm(const fluxb_int4_gemm_t* args);
+
 #ifdef __cplusplus
 }
 #endif

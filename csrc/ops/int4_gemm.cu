@@ -1,0 +1,164 @@
+// Host side of the products with 4-bit weights: layout of the weights, argument checks, choice of the kernel, launches.
+#include "../sm100/gemm_int4.cuh"
+
+#include "../runtime/host_common.h"
+
+#include <atomic>
+
+namespace fluxb {
+extern std::atomic<uint64_t> g_launches;
+
+namespace {
+
+// One thread per word: two 16-bit reads (four neighbouring values of rows g and g + 8), one 32-bit write.
+__global__ void int4_layout_kernel(const fluxb_int4_layout_t a, int Np, int Kp, int64_t words) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t units = Kp / 64;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < words; i += stride) {
+    const int s = static_cast<int>(i % 4), lane = static_cast<int>(i / 4 % 32);
+    const int64_t u = i / 128 % units, rest = i / 128 / units;
+    const int block = static_cast<int>(rest % (Np / 16)), e = static_cast<int>(rest / (Np / 16));
+    const int k = static_cast<int>(u) * 64 + s * 16 + lane % 4 * 4;
+    uint32_t word = 0;
+    for (int h = 0; h < 2; ++h) {
+      const int n = block * 16 + lane / 4 + h * 8;
+      uint32_t v = 0x8888u;                                      // (with zero points: the scale of zero makes them zero)
+      if (n < a.N && k < a.K)
+        v = *reinterpret_cast<const uint16_t*>(a.q + (static_cast<int64_t>(e) * a.N + n) * (a.K / 2) + k / 2);
+      word |= ((v & 0xfu) | (v >> 8 & 0xfu) << 4 | (v >> 4 & 0xfu) << 16 | (v >> 12 & 0xfu) << 20) << (8 * h);
+    }
+    static_cast<uint32_t*>(a.packed)[i] = word;
+  }
+}
+
+__global__ void int4_layout_scales_kernel(const fluxb_int4_layout_t a, int Np, int Kp, int G, int64_t count) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int groups = Kp / G, given = a.K / a.group;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count; i += stride) {
+    const int n = static_cast<int>(i % Np), j = static_cast<int>(i / Np % groups), e = static_cast<int>(i / Np / groups);
+    const int64_t to = (static_cast<int64_t>(e) * groups + j) * Np + n / 64 * 64 + int4_scale_slot(n % 64);
+    const bool in = n < a.N && j * G < a.K;
+    const int64_t from = (static_cast<int64_t>(e) * a.N + n) * given + static_cast<int64_t>(j) * G / a.group;
+    static_cast<uint16_t*>(a.scales_out)[to] = in ? static_cast<const uint16_t*>(a.scales)[from] : 0;
+    if (a.zeros_out != nullptr) a.zeros_out[to] = in ? a.zeros[from] & 15 : 8;
+  }
+}
+
+template <bool F16, int G, int NT>
+int launch_small(const Int4Params& p, cudaStream_t stream) {
+  using Cfg = Int4SmallCfg<NT>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  FLUXB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    FLUXB_CUDA_OK(cudaFuncSetAttribute(int4_small_kernel<F16, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg::SMEM_BYTES));
+    if (dev < 64) configured[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.E) * p.tiles * p.splits_k, 1, 1);
+  cfg.blockDim = dim3(kInt4Warps * 32, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits_k;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.splits_k > 1 ? 1 : 0;
+  FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_small_kernel<F16, G, NT>, p));
+  FLUXB_CUDA_OK(cudaGetLastError());
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return kOk;
+}
+
+template <bool F16, int G>
+int launch_small(const Int4Params& p, int64_t rows, cudaStream_t stream) {
+  if (rows <= 8) return launch_small<F16, G, 1>(p, stream);
+  if (rows <= 16) return launch_small<F16, G, 2>(p, stream);
+  return launch_small<F16, G, 4>(p, stream);
+}
+
+template <bool F16>
+int launch_small(const Int4Params& p, int G, int64_t rows, cudaStream_t stream) {
+  if (G == 32) return launch_small<F16, 32>(p, rows, stream);
+  if (G == 64) return launch_small<F16, 64>(p, rows, stream);
+  return launch_small<F16, 128>(p, rows, stream);
+}
+
+int round128(int v) { return (v + 127) / 128 * 128; }
+
+bool shape_ok(int experts, int N, int K, int group) {
+  return experts >= 1 && experts <= 512 && N >= 1 && N <= (1 << 24) && K >= 32 && K <= (1 << 24) &&
+         (group == 32 || group == 64 || (group >= 128 && group % 128 == 0)) && K % group == 0;
+}
+
+}  // namespace
+}  // namespace fluxb
+
+using namespace fluxb;
+
+extern "C" int fluxb_int4_layout(const fluxb_int4_layout_t* a) {
+  FLUXB_REQUIRE(a && a->q && a->scales && a->packed && a->scales_out, "null arguments");
+  FLUXB_REQUIRE((a->zeros != nullptr) == (a->zeros_out != nullptr), "zero points need both arrays");
+  FLUXB_REQUIRE(shape_ok(a->experts, a->N, a->K, a->group), "4-bit weights: sizes");
+  FLUXB_REQUIRE((reinterpret_cast<uintptr_t>(a->q) & 1) == 0 && (reinterpret_cast<uintptr_t>(a->packed) & 15) == 0 &&
+                    (reinterpret_cast<uintptr_t>(a->scales_out) & 15) == 0 && (reinterpret_cast<uintptr_t>(a->zeros_out) & 15) == 0,
+                "4-bit weights: alignment");
+  const int Np = round128(a->N), Kp = round128(a->K), G = a->group < 128 ? a->group : 128;
+  const int64_t words = static_cast<int64_t>(a->experts) * Np * (Kp / 8);
+  const int64_t count = static_cast<int64_t>(a->experts) * (Kp / G) * Np;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+  int sms = 0, rc;
+  if ((rc = device_sm_count(&sms))) return rc;
+  int4_layout_kernel<<<sms * 8, 256, 0, stream>>>(*a, Np, Kp, words);
+  int4_layout_scales_kernel<<<sms * 8, 256, 0, stream>>>(*a, Np, Kp, G, count);
+  FLUXB_CUDA_OK(cudaGetLastError());
+  g_launches.fetch_add(2, std::memory_order_relaxed);
+  return kOk;
+}
+
+extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
+  FLUXB_REQUIRE(a != nullptr, "null arguments");
+  FLUXB_REQUIRE(shape_ok(a->experts, a->N, a->K, a->group), "4-bit product: sizes");
+  FLUXB_REQUIRE(a->splits != nullptr || a->experts == 1, "several experts need their row counts");
+  FLUXB_REQUIRE(a->M >= 0 && a->M < (1ll << 31), "4-bit product: rows");
+  if (a->M == 0) return kOk;
+  FLUXB_REQUIRE(a->x && a->packed && a->scales && a->out, "null tensors");
+  FLUXB_REQUIRE(a->dtype == FLUXB_BF16 || a->dtype == FLUXB_FP16, "activations must be bf16 or fp16");
+  FLUXB_REQUIRE(a->scale_dtype == FLUXB_BF16 || a->scale_dtype == FLUXB_FP16, "scales must be bf16 or fp16");
+  FLUXB_REQUIRE(((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->packed) |
+                  reinterpret_cast<uintptr_t>(a->scales) | reinterpret_cast<uintptr_t>(a->zeros)) & 15) == 0,
+                "4-bit product: 16-byte aligned tensors");
+  FLUXB_REQUIRE(a->ldx % 8 == 0 && a->ldx >= 0 && a->ldo >= 0, "rows of the activations must be 16-byte aligned");
+  Int4Params p = {};
+  p.x = static_cast<const uint16_t*>(a->x);
+  p.packed = static_cast<const uint4*>(a->packed);
+  p.scales = static_cast<const uint16_t*>(a->scales);
+  p.zeros = a->zeros;
+  p.bias = static_cast<const uint16_t*>(a->bias);
+  p.splits = a->splits;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.M = a->M;
+  p.ldx = a->ldx;
+  p.ldo = a->ldo;
+  p.E = a->experts;
+  p.N = a->N;
+  p.K = a->K;
+  p.Np = round128(a->N);
+  p.Kp = round128(a->K);
+  p.scale_f16 = a->scale_dtype == FLUXB_FP16;
+  p.tiles = (a->N + 63) / 64;
+  int sms = 0, rc;
+  if ((rc = device_sm_count(&sms))) return rc;
+  const int64_t items = static_cast<int64_t>(p.E) * p.tiles;
+  FLUXB_REQUIRE(items * 8 < (1ll << 31), "4-bit product: too many tiles");
+  int s = 1;
+  while (s < 8 && items * s < 2ll * sms && p.Kp / 128 >= 2 * s * kInt4Warps) s *= 2;
+  p.splits_k = s;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
+  const int G = a->group < 128 ? a->group : 128;
+  const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;
+  return a->dtype == FLUXB_FP16 ? launch_small<true>(p, G, rows, stream) : launch_small<false>(p, G, rows, stream);
+}

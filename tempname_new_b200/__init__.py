@@ -23,6 +23,9 @@ from .ops.ag_gemm import AGKernel  # noqa: F401
 from .ops.quantization import Quantization  # noqa: F401
 from .ops.misc import (InplaceCast, bitwise_check, calc_scatter_index, inplace_cast_fp32_to_bf16,  # noqa: F401
                        moe_index_build, uniform_initialize)
+from .ops.route import moe_route  # noqa: F401
+from .ops.gated import gated_act  # noqa: F401
+from .ops.int4 import Int4Gemm, Int4GemmGrouped, dequantize_int4, quantize_int4  # noqa: F401
 from .ops.blockscale_gemm import BlockScaleGemm, blockscale_gemm_torch  # noqa: F401
 from .ops.ulysses import AllToAllTransposeGemm, GemmAllToAllTranspose  # noqa: F401
 from .ops.moe import (GemmGroupedV2, GemmGroupedV2AGScatterOp, GemmGroupedV2GatherRSOp, GemmGroupedV3,  # noqa: F401

@@ -2,6 +2,7 @@
 GemmRS."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional, Sequence
@@ -65,6 +66,14 @@ def current_stream_ptr(device=None) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index if isinstance(device, torch.device) else device
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_guard(device: torch.device):
+    """A context in which ``device`` is the current one, as launches of the runtime API need it (no cost where it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def fill_ptrs(arr, ptrs: Optional[Sequence[int]]) -> None:

@@ -1,0 +1,184 @@
+"""``moe_route``: the choice of a token's experts and their weights from the router's logits, with the gradient of the
+weights. It stands in front of ``moe_index_build``, which sorts the choices; the reference's tests use a softmax and a
+top-k of the framework there (``python/flux/testing/moe_utils.py``). The kernel and the definition are in
+``csrc/aux/route.cu``; ``moe_route_torch`` states the same in PyTorch (CPU path and test oracle)."""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+from ._dense import current_stream_ptr, device_guard, dtype_code
+
+_VP = ctypes.c_void_p
+_SCORES = {"softmax": 0, "sigmoid": 1}
+MAX_EXPERTS, MAX_TOPK, MAX_GROUPS = 512, 32, 32
+
+
+class RouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", _VP), ("bias", _VP), ("experts", _VP), ("weights", _VP), ("grad", _VP), ("dlogits", _VP),
+        ("tokens", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("num_experts", ctypes.c_int32), ("topk", ctypes.c_int32),
+        ("num_groups", ctypes.c_int32), ("topk_groups", ctypes.c_int32), ("group_top", ctypes.c_int32),
+        ("score", ctypes.c_int32), ("renormalize", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("stream", _VP),
+    ]
+
+
+def _order(values: torch.Tensor) -> torch.Tensor:
+    """Places of a row's values, largest first, ties to the lowest place, NaN last of all."""
+    lowest = torch.where(torch.isnan(values), torch.full_like(values, -math.inf), values)
+    # (two stable sorts: NaN behind -inf)
+    first = lowest.sort(dim=-1, descending=True, stable=True).indices
+    return first.gather(-1, torch.isnan(values).gather(-1, first).sort(dim=-1, stable=True).indices)
+
+
+def _choose_torch(logits, topk, score_func, bias, num_groups, topk_groups, group_top):
+    x = logits.double()
+    t, e = x.shape
+    masked = (x.amax(dim=1, keepdim=True) == -math.inf) if e else None
+    if score_func == "softmax":
+        score = torch.where(masked, torch.zeros_like(x), torch.softmax(x, dim=1))
+    else:
+        score = torch.sigmoid(x)
+    if bias is not None:
+        choice = by_group = score + bias.double()
+    else:
+        choice, by_group = x, (score if group_top == 2 else x)
+    if num_groups > 1:
+        size = e // num_groups
+        split = by_group.view(t, num_groups, size)
+        best = split.gather(2, _order(split)[:, :, :group_top]).sum(dim=2)
+        kept = torch.zeros(t, num_groups, dtype=torch.bool, device=x.device)
+        kept.scatter_(1, _order(best)[:, :topk_groups], True)
+        # (candidates in front of the others, whatever their values)
+        out = ~kept.repeat_interleave(size, dim=1)
+        first = _order(choice)
+        order = first.gather(1, out.gather(1, first).sort(dim=1, stable=True).indices)
+    else:
+        order = _order(choice)
+    return order[:, :topk]
+
+
+def moe_route_torch(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias: Optional[torch.Tensor] = None,
+                    num_groups: int = 1, topk_groups: int = 1, group_top: int = 1, renormalize: bool = True,
+                    scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The operator in PyTorch, differentiable by autograd; scores and sums in 64 bits."""
+    with torch.no_grad():
+        experts = _choose_torch(logits.detach(), topk, score_func, bias, num_groups, topk_groups, group_top)
+    x = logits.double()
+    picked = x.gather(1, experts)
+    none = x.detach().amax(dim=1, keepdim=True) == -math.inf
+    if score_func == "softmax":
+        # (rows without an expert: any finite numbers, replaced by zeros below)
+        x = torch.where(none, torch.zeros_like(x), x)
+        w = torch.softmax(x, dim=1).gather(1, experts)
+        if renormalize:
+            nan = torch.isnan(x.detach()).any(dim=1, keepdim=True)
+            safe = torch.where(none, torch.zeros_like(picked), picked)
+            w = torch.where(nan, torch.full_like(w, math.nan), torch.softmax(safe, dim=1))
+    else:
+        none = picked.detach().amax(dim=1, keepdim=True) == -math.inf
+        picked = torch.where(none, torch.zeros_like(picked), picked)
+        log = torch.nn.functional.logsigmoid(picked)
+        w = torch.softmax(log, dim=1) if renormalize else log.exp()
+    w = torch.where(none, torch.zeros_like(w), w)
+    return experts.to(torch.int32), (w * scale).float()
+
+
+def _args(logits, experts, weights, cfg) -> RouteArgs:
+    topk, score, _, groups, topk_groups, group_top, renorm, scale = cfg
+    a = RouteArgs()
+    a.logits, a.row_stride, a.dtype = logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype)
+    a.experts, a.weights = experts.data_ptr(), weights.data_ptr()
+    a.tokens, a.num_experts = logits.shape
+    a.topk, a.num_groups, a.topk_groups, a.group_top = topk, groups, topk_groups, group_top
+    a.score, a.renormalize, a.scale = _SCORES[score], int(renorm), scale
+    a.stream = current_stream_ptr(logits.device)
+    return a
+
+
+def _forward(logits, cfg):
+    x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
+    experts = torch.empty((x.shape[0], cfg[0]), dtype=torch.int32, device=x.device)
+    weights = torch.empty((x.shape[0], cfg[0]), dtype=torch.float32, device=x.device)
+    with device_guard(x.device):
+        a = _args(x, experts, weights, cfg)
+        if cfg[2] is not None:
+            a.bias = cfg[2].data_ptr()
+        _native.check(_native.lib().fluxb_moe_route(ctypes.byref(a)), "fluxb_moe_route")
+    return x, experts, weights
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, cfg):
+        x, experts, weights = _forward(logits, cfg)
+        ctx.save_for_backward(x, experts, weights)
+        ctx.cfg = cfg
+        ctx.mark_non_differentiable(experts)
+        return experts, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, grad):
+        x, experts, weights = ctx.saved_tensors
+        grad = grad.to(torch.float32).contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        with device_guard(x.device):
+            a = _args(x, experts, weights, ctx.cfg)
+            a.grad, a.dlogits = grad.data_ptr(), dx.data_ptr()
+            _native.check(_native.lib().fluxb_moe_route_bwd(ctypes.byref(a)), "fluxb_moe_route_bwd")
+        return dx, None
+
+
+def moe_route(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias: Optional[torch.Tensor] = None,
+              num_groups: int = 1, topk_groups: int = 1, group_top: int = 1, renormalize: bool = True,
+              scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(choosed_experts [tokens, topk] int32, weights [tokens, topk] float32)`` from ``logits [tokens, experts]``.
+
+    The scores are the softmax of a row or the sigmoid of each logit (``score_func``). ``bias [experts]`` (float32, no
+    gradient) is added to them for the choice only. With ``num_groups`` groups of consecutive experts, the
+    ``topk_groups`` groups whose ``group_top`` (1 or 2) best experts have the largest sum stay. Experts come best first,
+    equal ones by their index. The weights are the chosen experts' scores, divided by their sum (``renormalize``), times
+    ``scale``; they carry the gradient to the logits. An expert whose logit is -inf is chosen only when no other is left,
+    with weight 0; NaN ranks lowest and shows in the weights."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    E = logits.shape[1]
+    topk, num_groups, topk_groups, group_top = int(topk), int(num_groups), int(topk_groups), int(group_top)
+    if score_func not in _SCORES:
+        raise ValueError(f"score_func must be one of {tuple(_SCORES)}, got {score_func!r}")
+    if E > MAX_EXPERTS:
+        raise ValueError(f"at most {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= num_groups <= MAX_GROUPS or E % num_groups:
+        raise ValueError(f"{E} experts do not divide over {num_groups} groups (at most {MAX_GROUPS})")
+    if not 1 <= topk_groups <= num_groups:
+        raise ValueError("topk_groups must be between 1 and num_groups")
+    if group_top not in (1, 2) or (num_groups > 1 and group_top > E // num_groups):
+        raise ValueError("group_top must be 1 or 2, and no more than the experts of a group")
+    if not 1 <= topk <= min(MAX_TOPK, E // num_groups * topk_groups):
+        raise ValueError(f"topk must be between 1 and {min(MAX_TOPK, E // num_groups * topk_groups)}, got {topk}")
+    scale = float(scale)
+    if scale == 0.0 or not math.isfinite(ctypes.c_float(scale).value) or ctypes.c_float(scale).value == 0.0:
+        raise ValueError("scale must be finite and not zero")
+    if bias is not None:
+        if bias.shape != (E,) or bias.dtype != torch.float32 or bias.device != logits.device:
+            raise ValueError("bias must be float32 [experts] on the device of the logits")
+        bias = bias.detach().contiguous()
+    if num_groups == 1:
+        topk_groups = group_top = 1
+    if not logits.is_cuda:
+        return moe_route_torch(logits, topk, score_func, bias, num_groups, topk_groups, group_top, renormalize, scale)
+    cfg = (topk, score_func, bias, num_groups, topk_groups, group_top, bool(renormalize), scale)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Route.apply(logits, cfg)
+    return _forward(logits, cfg)[1:]
