@@ -1,7 +1,5 @@
 // Host side of the products with 4-bit weights: layout of the weights, argument checks, choice of the kernel, launches.
-#include "../sm100/gemm_int4.cuh"
-
-#include "../runtime/host_common.h"
+#include "int4_tile.h"
 
 #include <atomic>
 
@@ -149,16 +147,32 @@ extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
   p.Np = round128(a->N);
   p.Kp = round128(a->K);
   p.scale_f16 = a->scale_dtype == FLUXB_FP16;
-  p.tiles = (a->N + 63) / 64;
   int sms = 0, rc;
   if ((rc = device_sm_count(&sms))) return rc;
-  const int64_t items = static_cast<int64_t>(p.E) * p.tiles;
-  FLUXB_REQUIRE(items * 8 < (1ll << 31), "4-bit product: too many tiles");
-  int s = 1;
-  while (s < 8 && items * s < 2ll * sms && p.Kp / 128 >= 2 * s * kInt4Warps) s *= 2;
-  p.splits_k = s;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   const int G = a->group < 128 ? a->group : 128;
-  const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;
-  return a->dtype == FLUXB_FP16 ? launch_small<true>(p, G, rows, stream) : launch_small<false>(p, G, rows, stream);
+  const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;      // of an expert, on average
+  const int steps = p.Kp / 128;
+  if (rows <= 16) {
+    p.tiles = (a->N + 63) / 64;
+    const int64_t items = static_cast<int64_t>(p.E) * p.tiles;
+    FLUXB_REQUIRE(items * 8 < (1ll << 31), "4-bit product: too many tiles");
+    int s = 1;
+    while (s < 8 && items * s < 2ll * sms && steps >= 2 * s * kInt4Warps) s *= 2;
+    p.splits_k = s;
+    return a->dtype == FLUXB_FP16 ? launch_small<true>(p, G, rows, stream) : launch_small<false>(p, G, rows, stream);
+  }
+  Int4TileParams tp = {};
+  p.tiles = p.Np / 128;
+  const int tok = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  const int64_t items = ((a->M + tok - 1) / tok + (a->splits ? p.E : 0)) * p.tiles;
+  FLUXB_REQUIRE(items < (1ll << 31), "4-bit product: too many tiles");
+  p.splits_k = 1;
+  while (p.splits_k < 8 && (p.splits_k + 1) * items <= sms && steps >= 2 * (p.splits_k + 1)) ++p.splits_k;
+  tp.p = p;
+  tp.out_vec = a->ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(a->out) & 15) == 0;
+  tp.timeout_ns = 2000000000ull;
+  tp.status = reinterpret_cast<Status*>(a->status);
+  const int grid = p.splits_k > 1 ? static_cast<int>(items) * p.splits_k : static_cast<int>(items < sms ? items : sms);
+  return a->dtype == FLUXB_FP16 ? int4_tile_f16(tp, tok, G, grid, stream) : int4_tile_bf16(tp, tok, G, grid, stream);
 }
