@@ -424,7 +424,7 @@ typedef struct {
   const uint8_t* q;          /* [E, N, K / 2]: value 2j in the low half of byte j */
   const void* scales;        /* [E, N, K / group], bf16 | fp16 */
   const uint8_t* zeros;      /* [E, N, K / group] in 0 .. 15, or null: 8 */
-  void* packed;              /* [E][Np / 16][Kp / 64][512 bytes], Np and Kp: N and K rounded up to 128; 16-byte aligned */
+  void* packed;              /* [E][Np / 128][Kp / 128][8 KB], Np and Kp: N and K rounded up to 128; 16-byte aligned */
   void* scales_out;          /* [E][Kp / min(group, 128)][Np], 16 bits each; 16-byte aligned */
   uint8_t* zeros_out;        /* the same in bytes; null without zeros */
   int32_t experts, N, K, group;

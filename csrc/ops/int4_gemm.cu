@@ -11,12 +11,13 @@ namespace {
 // One thread per word: two 16-bit reads (four neighbouring values of rows g and g + 8), one 32-bit write.
 __global__ void int4_layout_kernel(const fluxb_int4_layout_t a, int Np, int Kp, int64_t words) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t units = Kp / 64;
+  const int64_t blocks = Kp / 128;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < words; i += stride) {
-    const int s = static_cast<int>(i % 4), lane = static_cast<int>(i / 4 % 32);
-    const int64_t u = i / 128 % units, rest = i / 128 / units;
-    const int block = static_cast<int>(rest % (Np / 16)), e = static_cast<int>(rest / (Np / 16));
-    const int k = static_cast<int>(u) * 64 + s * 16 + lane % 4 * 4;
+    const int s = static_cast<int>(i % 4), lane = static_cast<int>(i / 4 % 32), u = static_cast<int>(i / 128 % 2);
+    const int64_t rest = i / 2048;
+    const int kb = static_cast<int>(rest % blocks), nb = static_cast<int>(rest / blocks % (Np / 128));
+    const int block = nb * 8 + static_cast<int>(i / 256 % 8), e = static_cast<int>(rest / blocks / (Np / 128));
+    const int k = kb * 128 + u * 64 + s * 16 + lane % 4 * 4;
     uint32_t word = 0;
     for (int h = 0; h < 2; ++h) {
       const int n = block * 16 + lane / 4 + h * 8;
@@ -42,19 +43,19 @@ __global__ void int4_layout_scales_kernel(const fluxb_int4_layout_t a, int Np, i
   }
 }
 
-template <bool F16, int G, int NT>
+template <bool F16, bool SF16, int G, int NT>
 int launch_small(const Int4Params& p, cudaStream_t stream) {
-  using Cfg = Int4SmallCfg<NT>;
+  using Cfg = Int4SmallCfg<G, NT>;
   static bool configured[64] = {false};
   int dev = 0;
   FLUXB_CUDA_OK(cudaGetDevice(&dev));
   if (dev >= 64 || !configured[dev]) {
-    FLUXB_CUDA_OK(cudaFuncSetAttribute(int4_small_kernel<F16, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    FLUXB_CUDA_OK(cudaFuncSetAttribute(int4_small_kernel<F16, SF16, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Cfg::SMEM_BYTES));
     if (dev < 64) configured[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.E) * p.tiles * p.splits_k, 1, 1);
+  cfg.gridDim = dim3(p.tiles * p.splits_k, 1, 1);
   cfg.blockDim = dim3(kInt4Warps * 32, 1, 1);
   cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = stream;
@@ -65,24 +66,28 @@ int launch_small(const Int4Params& p, cudaStream_t stream) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.splits_k > 1 ? 1 : 0;
-  FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_small_kernel<F16, G, NT>, p));
+  FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_small_kernel<F16, SF16, G, NT>, p));
   FLUXB_CUDA_OK(cudaGetLastError());
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return kOk;
 }
 
-template <bool F16, int G>
+template <bool F16, bool SF16, int G>
 int launch_small(const Int4Params& p, int64_t rows, cudaStream_t stream) {
-  if (rows <= 8) return launch_small<F16, G, 1>(p, stream);
-  if (rows <= 16) return launch_small<F16, G, 2>(p, stream);
-  return launch_small<F16, G, 4>(p, stream);
+  if (rows <= 8) return launch_small<F16, SF16, G, 1>(p, stream);
+  return launch_small<F16, SF16, G, 2>(p, stream);
+}
+
+template <bool F16, bool SF16>
+int launch_small(const Int4Params& p, int G, int64_t rows, cudaStream_t stream) {
+  if (G == 32) return launch_small<F16, SF16, 32>(p, rows, stream);
+  if (G == 64) return launch_small<F16, SF16, 64>(p, rows, stream);
+  return launch_small<F16, SF16, 128>(p, rows, stream);
 }
 
 template <bool F16>
 int launch_small(const Int4Params& p, int G, int64_t rows, cudaStream_t stream) {
-  if (G == 32) return launch_small<F16, 32>(p, rows, stream);
-  if (G == 64) return launch_small<F16, 64>(p, rows, stream);
-  return launch_small<F16, 128>(p, rows, stream);
+  return p.scale_f16 ? launch_small<F16, true>(p, G, rows, stream) : launch_small<F16, false>(p, G, rows, stream);
 }
 
 int round128(int v) { return (v + 127) / 128 * 128; }
@@ -153,26 +158,25 @@ extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
   const int G = a->group < 128 ? a->group : 128;
   const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;      // of an expert, on average
   const int steps = p.Kp / 128;
-  if (rows <= 16) {
+  if (a->splits == nullptr && rows <= 16) {
     p.tiles = (a->N + 63) / 64;
-    const int64_t items = static_cast<int64_t>(p.E) * p.tiles;
-    FLUXB_REQUIRE(items * 8 < (1ll << 31), "4-bit product: too many tiles");
     int s = 1;
-    while (s < 8 && items * s < 2ll * sms && steps >= 2 * s * kInt4Warps) s *= 2;
+    while (s < 4 && 2 * s * p.tiles <= 2 * sms && steps >= 16 * s) s *= 2;
     p.splits_k = s;
     return a->dtype == FLUXB_FP16 ? launch_small<true>(p, G, rows, stream) : launch_small<false>(p, G, rows, stream);
   }
   Int4TileParams tp = {};
   p.tiles = p.Np / 128;
-  const int tok = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  const int tok = rows <= (a->splits ? 24 : 32) ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
   const int64_t items = ((a->M + tok - 1) / tok + (a->splits ? p.E : 0)) * p.tiles;
   FLUXB_REQUIRE(items < (1ll << 31), "4-bit product: too many tiles");
+  const int resident = sms * (tok == 32 ? 2 : 1);
   p.splits_k = 1;
-  while (p.splits_k < 8 && (p.splits_k + 1) * items <= sms && steps >= 2 * (p.splits_k + 1)) ++p.splits_k;
+  while (p.splits_k < 8 && (p.splits_k + 1) * items <= resident && steps >= 2 * (p.splits_k + 1)) ++p.splits_k;
   tp.p = p;
   tp.out_vec = a->ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(a->out) & 15) == 0;
   tp.timeout_ns = 2000000000ull;
   tp.status = reinterpret_cast<Status*>(a->status);
-  const int grid = p.splits_k > 1 ? static_cast<int>(items) * p.splits_k : static_cast<int>(items < sms ? items : sms);
+  const int grid = p.splits_k > 1 ? static_cast<int>(items) * p.splits_k : static_cast<int>(items < resident ? items : resident);
   return a->dtype == FLUXB_FP16 ? int4_tile_f16(tp, tok, G, grid, stream) : int4_tile_bf16(tp, tok, G, grid, stream);
 }

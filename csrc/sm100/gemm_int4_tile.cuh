@@ -10,11 +10,12 @@
 // rows. Smaller TOK alternate two accumulators between groups.
 //
 //   warps 0 .. 7    sums: TMEM lanes 32 (warp % 4), the first or second half of the columns (warp / 4); epilogue
-//   warps 8 .. 11   weights: packed words by cp.async into a ring of their own (a lane reads back what it copied, so the
-//                   ring needs no barriers), unpacked into TMEM
-//   warp 12         TMA of x, warp 13 MMA issue
-// One CTA per SM walks the tiles of all experts; the loads of a tile run ahead into the one before. With splits_k > 1 a
-// cluster shares one tile, each CTA with its part of k, and the sums meet in distributed shared memory in rank order.
+//                   (TOK = 32: warps 0 .. 3)
+//   the next 4 (8)  unpack the weights into TMEM
+//   the next three  loads of x and scales, MMA issue, loads of packed weights and zero points
+// One CTA per SM (two with TOK = 32) walks the tiles of all experts; the loads of a tile run ahead into the one before. With
+// splits_k > 1 a cluster shares one tile, each CTA with its part of k, and the sums meet in distributed shared memory in rank
+// order.
 #pragma once
 
 #include "gemm_int4.cuh"
@@ -30,35 +31,63 @@ struct Int4TileParams {
 };
 
 constexpr int kInt4MaxExperts = 512;
+template <int I>
+struct IntC {
+  static constexpr int value = I;
+};
 
 template <int TOK_, int G_, bool F16_>
 struct Int4TileCfg {
   static constexpr int TOK = TOK_, G = G_;
   static constexpr bool F16 = F16_;
-  static constexpr int THREADS = 512;
   static constexpr int HALVES = TOK_ == 256 ? 2 : 1;
   static constexpr int NMMA = TOK_ / HALVES;
-  static constexpr int CPT = TOK_ / 2;                   // columns of a thread
-  static constexpr int GPS = 128 / G_;                   // groups per 128 columns of k
-  static constexpr int A_BUFS = 4, A_COL = 256;          // TMEM: accumulators in columns 0 .. 255, weights behind them
-  static constexpr int XS_BYTES = TOK_ * 128;            // one stage: 64 columns of k
-  static constexpr int X_STAGES = TOK_ == 256 ? 5 : TOK_ == 128 ? 6 : 12;
-  static constexpr int PF = TOK_ == 256 ? 4 : 8;         // blocks of 128 columns in the ring of packed weights
-  static constexpr int W_BYTES = PF * 8192, Z_BYTES = PF * GPS * 512;
-  static constexpr int EPI_BYTES = 2 * 16 * 128 * 4;     // 16 rows of the output at a time for each half
+  static constexpr int GPS = 128 / G_;                   // groups per block of 128 columns of k
+  // The smallest tiles wait for weights, and what a CTA does once per block (waits, issue) would hold them up: two CTAs share
+  // an SM. With TOK = 64, which needs the shared memory, two sets of warps unpack instead.
+  static constexpr int CTAS = TOK_ == 32 ? 2 : 1;
+  static constexpr int SUM_WARPS = CTAS == 2 ? 4 : 8, SETS = SUM_WARPS / 4, UNPACK_SETS = TOK_ == 64 ? 2 : 1;
+  static constexpr int UNPACK_WARP0 = SUM_WARPS, X_WARP = SUM_WARPS + 4 * UNPACK_SETS, MMA_WARP = X_WARP + 1,
+                       W_WARP = X_WARP + 2, TABLE_WARP = X_WARP + 3;
+  static constexpr int THREADS = 32 * (X_WARP + 4);
+  static constexpr int CPD = NMMA / SETS;                // columns of an accumulator that a thread reads
+  static constexpr int CPT = CPD * HALVES;               // columns that it sums
+  // TMEM: accumulators in the first half of the CTA's columns, blocks of weights in the second
+  static constexpr int TMEM_COLS = 512 / CTAS, A_COL = TMEM_COLS / 2, A_BUFS = A_COL / 64, D_BUFS = A_COL / NMMA;
+  // x arrives in blocks of 128 columns, with TOK = 256 in halves of a block (shared memory holds two and a half of them)
+  static constexpr int XS_PER_BLOCK = TOK_ == 256 ? 2 : 1;
+  static constexpr int XS_BYTES = TOK_ * 256 / XS_PER_BLOCK;
+  static constexpr int X_STAGES = TOK_ == 256 ? 5 : TOK_ == 64 ? 8 : 4;
+  // One commit per group or block hands its product over; the last one of a block also frees its weights and its x. The
+  // barriers are a ring of RING blocks. (TOK = 256: one barrier per half, and commits of their own for x and weights.)
+  static constexpr int RING = TOK_ == 256 ? 1 : X_STAGES;
+  // Groups that are handed over at once: those of a block where the accumulators hold two blocks, else one. (HALVES == 2:
+  // one half of one group.) A wait that finds its phase complete still costs a warp about 110 cycles.
+  static constexpr int GRAN = HALVES == 1 && D_BUFS >= 2 * GPS ? GPS : 1;
+  static constexpr int HPB = GPS / GRAN;                 // hand-overs per block (and half)
+  static constexpr int UNITS = HALVES == 2 ? 2 : D_BUFS / GRAN;
+  static constexpr int D_BARS = TOK_ == 256 ? 2 : RING * HPB;
+  static constexpr int SC_SLOTS = TOK_ == 256 ? 8 : RING + (D_BUFS + GPS - 1) / GPS;  // blocks of scales, see the x warp
+  static constexpr int SC_BYTES = GPS * 256;
+  static constexpr int W_STAGES = TOK_ == 64 ? 6 : TOK_ == 256 ? 3 : 4;        // blocks of packed weights and zero points
+  static constexpr int W_BYTES = 8192, Z_BYTES = GPS * 128;
+  static constexpr int EPI_PITCH = 36;                   // floats; a warp stages 16 rows of the output at a time
+  static constexpr int EPI_BYTES = SUM_WARPS * 16 * EPI_PITCH * 4;
   static constexpr int TAB_BYTES = (2 * (kInt4MaxExperts + 1) * 4 + 15) / 16 * 16;
-  static constexpr int BAR_BYTES = 512;
-  static constexpr int X_OFF = 0, W_OFF = X_STAGES * XS_BYTES, Z_OFF = W_OFF + W_BYTES, EPI_OFF = Z_OFF + Z_BYTES,
-                       TAB_OFF = EPI_OFF + EPI_BYTES, BAR_OFF = TAB_OFF + TAB_BYTES;
-  static constexpr int SMEM_BYTES = BAR_OFF + BAR_BYTES + 1024;
-  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+  static constexpr int BAR_BYTES = 640;
+  static constexpr int X_OFF = 0, SC_OFF = X_STAGES * XS_BYTES, W_OFF = SC_OFF + SC_SLOTS * SC_BYTES,
+                       Z_OFF = W_OFF + W_STAGES * W_BYTES, TAB_OFF = Z_OFF + W_STAGES * Z_BYTES,
+                       BAR_OFF = TAB_OFF + TAB_BYTES, END = BAR_OFF + BAR_BYTES;
+  static constexpr int EPI_OFF = END;
+  static constexpr int SMEM_BYTES = EPI_OFF + EPI_BYTES + 1024;
+  static_assert(CTAS * (SMEM_BYTES + 1024) <= 228 * 1024, "shared memory");
   static_assert(X_STAGES * XS_BYTES >= TOK_ * 512, "the staged tile of a split product reuses the ring");
 };
 
 template <class Cfg>
-__global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid_constant__ Int4TileParams tp) {
-  using H = int4::Half<Cfg::F16>;
-  constexpr int TOK = Cfg::TOK, G = Cfg::G, GPS = Cfg::GPS, NMMA = Cfg::NMMA, CPT = Cfg::CPT;
+__global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(const __grid_constant__ Int4TileParams tp) {
+  constexpr int TOK = Cfg::TOK, G = Cfg::G, GPS = Cfg::GPS, GRAN = Cfg::GRAN, HPB = Cfg::HPB;
+  constexpr int NMMA = Cfg::NMMA, CPD = Cfg::CPD, CPT = Cfg::CPT;
   extern __shared__ uint8_t smem_raw[];
   const Int4Params& p = tp.p;
   const uint32_t raw = ptx::smem_u32(smem_raw);
@@ -67,12 +96,15 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
   uint8_t* const sm = smem_raw + pad;
   auto bar = [&](int i) { return base + Cfg::BAR_OFF + 8u * i; };
   auto xfull = [&](int s) { return bar(s); };
-  auto xempty = [&](int s) { return bar(Cfg::X_STAGES + s); };
+  auto xempty = [&](int s) { return bar(Cfg::X_STAGES + s); };                 // (TOK = 256)
   auto afull = [&](int b) { return bar(2 * Cfg::X_STAGES + b); };
-  auto aempty = [&](int b) { return bar(2 * Cfg::X_STAGES + Cfg::A_BUFS + b); };
-  auto dfull = [&](int d) { return bar(2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + d); };
-  auto dempty = [&](int d) { return bar(2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + 2 + d); };
-  constexpr int kBars = 2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + 4;
+  auto aempty = [&](int b) { return bar(2 * Cfg::X_STAGES + Cfg::A_BUFS + b); };       // (TOK = 256)
+  auto dempty = [&](int d) { return bar(2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + d); };
+  auto dfull = [&](int d) { return bar(2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + Cfg::UNITS + d); };
+  constexpr int kWBar = 2 * Cfg::X_STAGES + 2 * Cfg::A_BUFS + Cfg::UNITS + Cfg::D_BARS;
+  auto wfull = [&](int s) { return bar(kWBar + s); };
+  auto wempty = [&](int s) { return bar(kWBar + Cfg::W_STAGES + s); };
+  constexpr int kBars = kWBar + 2 * Cfg::W_STAGES;
   static_assert(8 * kBars + 8 <= Cfg::BAR_BYTES, "barrier block too small");
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(sm + Cfg::BAR_OFF + 8 * kBars);
   volatile uint32_t* abort_word = tmem_slot + 1;
@@ -95,19 +127,21 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
       ptx::mbar_init(afull(b), 4);
       ptx::mbar_init(aempty(b), 1);
     }
-    for (int d = 0; d < 2; ++d) {
-      ptx::mbar_init(dfull(d), 1);
-      ptx::mbar_init(dempty(d), Cfg::HALVES == 2 ? 4 : 8);
+    for (int s = 0; s < Cfg::W_STAGES; ++s) {
+      ptx::mbar_init(wfull(s), 1);
+      ptx::mbar_init(wempty(s), 4);
     }
+    for (int d = 0; d < Cfg::UNITS; ++d) ptx::mbar_init(dempty(d), Cfg::SUM_WARPS);
+    for (int d = 0; d < Cfg::D_BARS; ++d) ptx::mbar_init(dfull(d), 1);
     *abort_word = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == 12 && lane == 0) ptx::prefetch_tmap(&tp.tm_x);
-  if (warp == 13) {
-    ptx::tmem_alloc<1>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+  if (warp == Cfg::X_WARP && lane == 0) ptx::prefetch_tmap(&tp.tm_x);
+  if (warp == Cfg::MMA_WARP) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<1>();
   }
-  if (warp == 14) {
+  if (warp == Cfg::TABLE_WARP) {
     // rows and tiles of the experts; negative counts are none, rows past the input do not exist
     int64_t rows = 0;
     int tiles = 0;
@@ -144,7 +178,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
   ptx::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const WaitCtx wc{tp.status, abort_word, tp.timeout_ns};
-  const int items = tile_of[p.E] * p.tiles;
+  const int items = __shfl_sync(0xffffffffu, tile_of[p.E], 0) * p.tiles;    // (known to be the same in all lanes)
   const int first = blockIdx.x / S, stride = gridDim.x / S;
 
   struct Item {
@@ -189,66 +223,65 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
     __syncwarp();
   };
 
-  if (warp < 8) {
+  if (warp < Cfg::SUM_WARPS) {
     // ------------------------------------------------------------------ sums and epilogue
     if constexpr (TOK == 256) ptx::setmaxnreg_inc<200>();
     const int set = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
-    const int groups = p.Kp / G, g0 = kb0 * GPS, ng = (kb1 - kb0) * GPS;
     const int slot = (r / 64) * 64 + int4_scale_slot(r % 64);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    float* const stage = reinterpret_cast<float*>(sm + Cfg::EPI_OFF) + set * (16 * 128);
-    uint32_t count = 0;          // groups so far
+    float* const stage = reinterpret_cast<float*>(sm + Cfg::EPI_OFF) + warp * (16 * Cfg::EPI_PITCH);
+    const uint16_t* const scales = reinterpret_cast<const uint16_t*>(sm + Cfg::SC_OFF) + slot;
+    uint32_t blocks = 0, blocks1 = 0;            // so far; with a second half
     bool ok = true;
-    uint16_t next[4];
-    auto fetch = [&](int item, int j) {          // scales of groups j .. j + 3
-      if (item >= items) return;
-      const Item it = item_of(item);
-      const uint16_t* s = p.scales + (static_cast<int64_t>(it.e) * groups + g0) * p.Np + it.n0 + slot;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) next[i] = j + i < ng ? s[static_cast<int64_t>(j + i) * p.Np] : static_cast<uint16_t>(0);
-    };
-    fetch(first, 0);
     for (int item = first; item < items && ok; item += stride) {
       const Item it = item_of(item);
       uint64_t acc[CPT / 2];
 #pragma unroll
       for (int i = 0; i < CPT / 2; ++i) acc[i] = 0ull;
-      for (int j0 = 0; j0 < ng && ok; j0 += 4) {
-        uint16_t now[4];
+      const bool both = it.last - it.row > NMMA;           // (TOK = 256) the second half has rows
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks, blocks1 += both) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) now[i] = next[i];
-        if (j0 + 4 < ng) fetch(item, j0 + 4);
-        else fetch(item + stride, 0);
+        for (int j = 0; j < GPS; ++j) {
+          float f = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (j0 + i >= ng) break;
-          const uint32_t d = Cfg::HALVES == 2 ? static_cast<uint32_t>(set) : count & 1u;
-          const uint32_t phase = Cfg::HALVES == 2 ? count & 1u : count >> 1 & 1u;
-          ++count;
-          const float f = ptx::half_bits_to_float(now[i], p.scale_f16);
-          const uint64_t ff = ptx::pack_f32x2(f, f);
-          if (!mbar_wait_warp(wc, dfull(d), phase, kSiteTmemFull)) {
-            ok = false;
-            break;
-          }
-          ptx::tc_fence_after();
-          const uint32_t at = lanes + (Cfg::HALVES == 2 ? set * NMMA : d * NMMA + set * CPT);
-          constexpr int W = CPT == 128 || CPT < 32 ? 16 : 32;  // (128 sums leave room for 16 more registers)
-#pragma unroll
-          for (int c = 0; c < CPT; c += W) {
-            uint32_t v[W];
-            if constexpr (W == 32) ptx::tmem_ld_32x32b_x32(at + c, v);
-            else ptx::tmem_ld_32x32b_x16(at + c, v);
-            ptx::tmem_ld_wait();
-            if (c + W == CPT) {
-              ptx::tc_fence_before();
-              __syncwarp();
-              if (lane == 0) ptx::mbar_arrive_relaxed(dempty(d));
+          for (int h = 0; h < Cfg::HALVES; ++h) {
+            if (h == 1 && !both) break;
+            // hand-overs so far (TOK = 256: of this half)
+            const uint32_t count = Cfg::HALVES == 2 ? (h == 0 ? blocks : blocks1) * GPS + j : blocks * HPB + j / GRAN;
+            const uint32_t unit = Cfg::HALVES == 2 ? static_cast<uint32_t>(h) : count % Cfg::UNITS;
+            const uint32_t d = unit * GRAN + j % GRAN;
+            if (j % GRAN == 0) {
+              const uint32_t full = Cfg::HALVES == 2 ? static_cast<uint32_t>(h) : count % Cfg::D_BARS;
+              const uint32_t phase = (Cfg::HALVES == 2 ? count : count / Cfg::D_BARS) & 1u;
+              if (!mbar_wait_all_warp(wc, MbarPhase{dfull(full), phase, kSiteTmemFull})) {
+                ok = false;
+                break;
+              }
+              ptx::tc_fence_after();
             }
+            if (h == 0)
+              f = ptx::half_bits_to_float(scales[(blocks % Cfg::SC_SLOTS) * (Cfg::SC_BYTES / 2) + j * 128], p.scale_f16);
+            const uint64_t ff = ptx::pack_f32x2(f, f);
+            const uint32_t at = lanes + d * NMMA + set * CPD;
+            constexpr int W = Cfg::CTAS == 2 ? 16 : 32;      // columns at a time, as registers allow
 #pragma unroll
-            for (int k = 0; k < W / 2; ++k)
-              acc[c / 2 + k] = ptx::ffma2(ptx::pack_b32x2(v[2 * k], v[2 * k + 1]), ff, acc[c / 2 + k]);
+            for (int c = 0; c < CPD; c += W) {
+              uint32_t v[W];
+              if constexpr (W == 32) ptx::tmem_ld_32x32b_x32(at + c, v);
+              else ptx::tmem_ld_32x32b_x16(at + c, v);
+              ptx::tmem_ld_wait(v);
+              if (c + W == CPD && j % GRAN == GRAN - 1) {
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(dempty(unit));
+              }
+#pragma unroll
+              for (int k = 0; k < W / 2; ++k)
+                acc[(h * CPD + c) / 2 + k] =
+                    ptx::ffma2(ptx::pack_b32x2(v[2 * k], v[2 * k + 1]), ff, acc[(h * CPD + c) / 2 + k]);
+            }
           }
+          if (!ok) break;
         }
       }
       if (!ok) break;
@@ -257,30 +290,35 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
         float* tile = reinterpret_cast<float*>(sm + Cfg::X_OFF);
 #pragma unroll
         for (int c = 0; c < CPT / 2; ++c) {
-          tile[(set * CPT + 2 * c) * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[c]));
-          tile[(set * CPT + 2 * c + 1) * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[c] >> 32));
+          const int m = c * 2 / CPD * NMMA + set * CPD + c * 2 % CPD;
+          tile[m * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[c]));
+          tile[(m + 1) * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[c] >> 32));
         }
         continue;
       }
-      const int live = it.last - it.row - set * CPT;       // rows of x that this half holds
+      // 16 rows of x by this warp's 32 rows of the weights, turned around in shared memory (nobody waits for other warps)
 #pragma unroll
       for (int c0 = 0; c0 < CPT; c0 += 16) {
-        if (c0 >= live) break;
+        const int m0 = c0 / CPD * NMMA + set * CPD + c0 % CPD;
+        const int live = it.last - it.row - m0;
+        if (live <= 0) break;
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
-          stage[c * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2]));
-          stage[(c + 1) * 128 + r] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2] >> 32));
+          stage[c * Cfg::EPI_PITCH + lane] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2]));
+          stage[(c + 1) * Cfg::EPI_PITCH + lane] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2] >> 32));
         }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + set) : "memory");
-        for (int u = quad * 32 + lane; u < 256; u += 128) {
-          const int m = u / 16, n = it.n0 + u % 16 * 8;
-          if (c0 + m >= live || n >= p.N) continue;
-          const float4 a = *reinterpret_cast<const float4*>(stage + m * 128 + u % 16 * 8);
-          const float4 b = *reinterpret_cast<const float4*>(stage + m * 128 + u % 16 * 8 + 4);
-          float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-          store8(v, static_cast<int64_t>(it.row) + set * CPT + c0 + m, n);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = i * 8 + lane / 4, n = it.n0 + quad * 32 + lane % 4 * 8;
+          if (m < live && n < p.N) {
+            const float4 a = *reinterpret_cast<const float4*>(stage + m * Cfg::EPI_PITCH + lane % 4 * 8);
+            const float4 b = *reinterpret_cast<const float4*>(stage + m * Cfg::EPI_PITCH + lane % 4 * 8 + 4);
+            float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            store8(v, static_cast<int64_t>(it.row) + m0 + m, n);
+          }
         }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + set) : "memory");
+        __syncwarp();
       }
     }
     ptx::tc_fence_before();
@@ -291,7 +329,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
       if (first < items) {
         const Item it = item_of(first);
         const int live = min(TOK, it.last - it.row);
-        for (int u = rank * 256 + static_cast<int>(threadIdx.x); u < live * 16; u += S * 256) {
+        for (int u = rank * (Cfg::SUM_WARPS * 32) + static_cast<int>(threadIdx.x); u < live * 16;
+             u += S * (Cfg::SUM_WARPS * 32)) {
           const int m = u / 16, n = it.n0 + u % 16 * 8;
           if (n >= p.N) continue;
           const uint32_t at = base + Cfg::X_OFF + (m * 128 + u % 16 * 8) * 4;
@@ -312,92 +351,83 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
     } else {
       __syncthreads();
     }
-  } else if (warp < 12) {
+  } else if (warp < Cfg::X_WARP) {
     // ------------------------------------------------------------------ weights
     if constexpr (TOK == 256) ptx::setmaxnreg_dec<72>();
-    const int q = warp - 8, g = lane >> 2;
-    const int64_t units = p.Kp / 64;
-    const int groups = p.Kp / G;
-    const uint32_t wring = base + Cfg::W_OFF + (q * 4 * 32 + lane) * 16;       // [PF][warp][4][lane]
-    const uint32_t zring = base + Cfg::Z_OFF + (q * GPS * 32 + lane) * 4;      // [PF][warp][GPS][lane]
-    int fetch_item = first, fetch_kb = kb0;
-    const uint4* wsrc = nullptr;
-    const uint8_t* zsrc = nullptr;
-    auto aim = [&] {
-      if (fetch_item >= items) return;
-      const Item it = item_of(fetch_item);
-      wsrc = p.packed + ((static_cast<int64_t>(it.e) * (p.Np / 16) + it.n0 / 16 + 2 * q) * units) * 32 + lane;
-      if (p.zeros != nullptr)
-        zsrc = p.zeros + static_cast<int64_t>(it.e) * groups * p.Np + it.n0 + (q / 2) * 64 + g * 8 + (q % 2) * 4;
+    const int q = (warp - Cfg::UNPACK_WARP0) & 3, turn = (warp - Cfg::UNPACK_WARP0) >> 2;    // blocks turn, turn + sets, ...
+    const uint32_t wring = base + Cfg::W_OFF + (q * 4 * 32 + lane) * 16;
+    const uint32_t zring = base + Cfg::Z_OFF + (q / 2) * 64 + (lane >> 2) * 8 + (q % 2) * 4;
+    const bool zeros = p.zeros != nullptr;
+    const uint32_t total = first < items ? static_cast<uint32_t>((items - 1 - first) / stride + 1) * (kb1 - kb0) : 0u;
+    // Half a block at a time (64 columns): its words are unpacked while the stores of the half before are on their way to
+    // TMEM, which are waited for (and, at the end of a block, published) just before the next ones are issued.
+    uint32_t last = 0;           // buffer whose stores are on their way
+    bool pending = false, ok = true;
+    auto publish = [&](uint32_t buf) {
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(afull(buf));
     };
-    auto fetch = [&](int slot) {                 // the next block, if there is one, into a slot of the ring
-      if (fetch_item < items) {
+    uint32_t slot = turn, wphase = 0;
+    for (uint32_t count = turn; count < total; count += Cfg::UNPACK_SETS) {
+      const uint32_t buf = count % Cfg::A_BUFS;
+      // the packed block is here, and what was multiplied from its place in TMEM is done
+      const uint32_t before = count - Cfg::A_BUFS;
+      const uint32_t done = Cfg::HALVES == 2 ? aempty(buf) : dfull(before % Cfg::RING * HPB + HPB - 1);
+      const uint32_t dphase = (Cfg::HALVES == 2 ? before / Cfg::A_BUFS : before / Cfg::RING) & 1u;
+      if (!mbar_wait_all_warp(wc, MbarPhase{wfull(slot), wphase, kSiteSmemFull})) break;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          ptx::cp_async_16(wring + slot * 8192 + i * 512, wsrc + ((i >> 1) * units + fetch_kb * 2 + (i & 1)) * 32, 16);
-        if (p.zeros != nullptr) {
+      for (int u = 0; u < 2; ++u) {
+        constexpr int GPH = G < 64 ? 64 / G : 1;             // groups of the half
+        uint32_t w[2][4], zz[GPH], a[2][16];
 #pragma unroll
-          for (int j = 0; j < GPS; ++j)
-            ptx::cp_async_4(zring + slot * (GPS * 512) + j * 128, zsrc + (static_cast<int64_t>(fetch_kb) * GPS + j) * p.Np);
-        }
-        if (++fetch_kb == kb1) {
-          fetch_kb = kb0;
-          fetch_item += stride;
-          aim();
-        }
-      }
-      ptx::cp_async_commit();
-    };
-    aim();
-    for (int s = 0; s < Cfg::PF; ++s) fetch(s);
-    int slot = 0;
-    uint32_t count = 0;
-    bool ok = true;
-    for (int item = first; item < items && ok; item += stride) {
-      for (int kb = kb0; kb < kb1; ++kb, ++count) {
-        ptx::cp_async_wait<Cfg::PF - 1>();
-        const uint32_t buf = count % Cfg::A_BUFS;
-        if (!mbar_wait_warp(wc, aempty(buf), (count / Cfg::A_BUFS & 1u) ^ 1u, kSiteTmemEmpty)) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        uint32_t zz[GPS];
-#pragma unroll
-        for (int j = 0; j < GPS; ++j) {
-          zz[j] = 0x08080808u;
-          if (p.zeros != nullptr)
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zz[j]) : "r"(zring + slot * (GPS * 512) + j * 128));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {            // row block i / 2 of the warp's two, 64 columns i % 2
-          uint32_t w[4];
+        for (int i = 0; i < 2; ++i)
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(wring + slot * 8192 + i * 512));
-          uint32_t a[16];
+                       : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                       : "r"(wring + slot * Cfg::W_BYTES + (2 * i + u) * 512));
+#pragma unroll
+        for (int j = 0; j < GPH; ++j) {
+          zz[j] = 0x08080808u;
+          if (zeros)
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zz[j]) : "r"(zring + slot * Cfg::Z_BYTES + (u * 64 / G + j) * 128));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                        // the warp's two row blocks
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const uint32_t z = zz[((i & 1) * 64 + s * 16) / G] >> (i >> 1) * 16;
-            const uint32_t z0 = H::kMagic + (z & 0xffu) * 0x00010001u;
-            const uint32_t z1 = H::kMagic + (z >> 8 & 0xffu) * 0x00010001u;
-            a[4 * s] = H::sub((w[s] & 0x000f000fu) | H::kMagic, z0);
-            a[4 * s + 1] = H::sub((w[s] >> 4 & 0x000f000fu) | H::kMagic, z0);
-            a[4 * s + 2] = H::sub((w[s] >> 8 & 0x000f000fu) | H::kMagic, z1);
-            a[4 * s + 3] = H::sub((w[s] >> 12 & 0x000f000fu) | H::kMagic, z1);
+            const uint32_t z = zz[s * 16 / G % GPH];
+            const uint32_t z0 = i == 0 ? int4::magic_zero<Cfg::F16, 0>(z) : int4::magic_zero<Cfg::F16, 2>(z);
+            const uint32_t z1 = i == 0 ? int4::magic_zero<Cfg::F16, 1>(z) : int4::magic_zero<Cfg::F16, 3>(z);
+            int4::unpack<Cfg::F16>(w[i][s], z0, z1, a[i][4 * s], a[i][4 * s + 1], a[i][4 * s + 2], a[i][4 * s + 3]);
           }
-          ptx::tmem_st_16x256b_x4(tmem + (static_cast<uint32_t>(q * 32 + (i >> 1) * 16) << 16) + Cfg::A_COL + buf * 64 + (i & 1) * 32,
-                                  a);
         }
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(afull(buf));
-        fetch(slot);
-        slot = slot + 1 == Cfg::PF ? 0 : slot + 1;
+        if (u == 0) {
+          if (pending) publish(last);
+          pending = false;
+          if (count >= Cfg::A_BUFS && !mbar_wait_all_warp(wc, MbarPhase{done, dphase, kSiteTmemEmpty})) {
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          ptx::tmem_st_16x256b_x4(
+              tmem + (static_cast<uint32_t>(q * 32 + i * 16) << 16) + Cfg::A_COL + buf * 64 + u * 32, a[i]);
+      }
+      if (!ok) break;
+      pending = true;
+      last = buf;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(wempty(slot));       // (the words have been read: they are in the stores)
+      slot += Cfg::UNPACK_SETS;
+      if (slot >= Cfg::W_STAGES) {
+        slot -= Cfg::W_STAGES;
+        wphase ^= 1u;
       }
     }
-    ptx::cp_async_wait<0>();
+    if (pending) publish(last);
     drain();
     if (S > 1) ptx::cluster_sync();
     else __syncthreads();
@@ -407,86 +437,194 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1) int4_tile_kernel(const __grid
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    if (warp == 12) {
+    if (warp == Cfg::X_WARP) {
       // ------------------------------------------------------------------ x
+      // Scales come along with x. They are read when the product is done, by when the stage of x may be in use again: their
+      // ring is longer. Block b is loaded when block b - RING has been multiplied, for which the groups D_BUFS before its
+      // last one had to be summed, and that many more blocks have slots of their own. (TOK = 256: x runs less than three
+      // blocks ahead, sums one behind.)
+      constexpr int PER = Cfg::XS_PER_BLOCK;
+      const int groups = p.Kp / G;
+      uint32_t blocks = 0;
       for (int item = first; item < items && ok; item += stride) {
         const Item it = item_of(item);
-        for (int u = 2 * kb0; u < 2 * kb1; ++u) {
-          if (!mbar_wait_warp(wc, xempty(stage), phase ^ 1u, kSiteSmemEmpty)) {
+        const uint16_t* const scales = p.scales + static_cast<int64_t>(it.e) * groups * p.Np + it.n0;
+        for (int u = PER * kb0; u < PER * kb1; ++u) {
+          const uint32_t empty = Cfg::HALVES == 2 ? xempty(stage) : dfull(stage * HPB + HPB - 1);
+          if (!mbar_wait_warp(wc, empty, phase ^ 1u, kSiteSmemEmpty)) {
             ok = false;
             break;
           }
           if (ptx::elect_one()) {
-            ptx::mbar_arrive_expect_tx(xfull(stage), Cfg::XS_BYTES);
-            ptx::tma_load_2d(base + Cfg::X_OFF + stage * Cfg::XS_BYTES, &tp.tm_x, xfull(stage), u * 64, it.row);
+            const uint32_t to = base + Cfg::X_OFF + stage * Cfg::XS_BYTES;
+            const bool block = PER == 1 || u % 2 == 0;       // (the first part of a block)
+            ptx::mbar_arrive_expect_tx(xfull(stage), Cfg::XS_BYTES + (block ? Cfg::SC_BYTES : 0));
+            ptx::tma_load_2d(to, &tp.tm_x, xfull(stage), u * (128 / PER), it.row);
+            if (PER == 1) ptx::tma_load_2d(to + Cfg::XS_BYTES / 2, &tp.tm_x, xfull(stage), u * 128 + 64, it.row);
+            if (block) {
+#pragma unroll
+              for (int j = 0; j < GPS; ++j)
+                ptx::bulk_load(base + Cfg::SC_OFF + (blocks % Cfg::SC_SLOTS) * Cfg::SC_BYTES + j * 256,
+                               scales + (static_cast<int64_t>(u / PER) * GPS + j) * p.Np, 256, xfull(stage));
+            }
           }
           __syncwarp();
+          if (PER == 1 || u % 2 == 1) ++blocks;
           if (++stage == Cfg::X_STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-    } else if (warp == 13) {
+    } else if (warp == Cfg::W_WARP) {
+      // ------------------------------------------------------------------ packed weights
+      const int groups = p.Kp / G;
+      for (int item = first; item < items && ok; item += stride) {
+        const Item it = item_of(item);
+        const uint8_t* const from = reinterpret_cast<const uint8_t*>(p.packed) +
+                                    (static_cast<int64_t>(it.e) * (p.Np / 128) + it.n0 / 128) * steps * Cfg::W_BYTES;
+        const uint8_t* const zfrom = p.zeros + static_cast<int64_t>(it.e) * groups * p.Np + it.n0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_all_warp(wc, MbarPhase{wempty(stage), phase ^ 1u, kSiteSmemEmpty})) {
+            ok = false;
+            break;
+          }
+          if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(wfull(stage), Cfg::W_BYTES + (p.zeros != nullptr ? Cfg::Z_BYTES : 0));
+            ptx::bulk_load(base + Cfg::W_OFF + stage * Cfg::W_BYTES, from + static_cast<int64_t>(kb) * Cfg::W_BYTES, Cfg::W_BYTES,
+                           wfull(stage));
+            if (p.zeros != nullptr) {
+#pragma unroll
+              for (int j = 0; j < GPS; ++j)
+                ptx::bulk_load(base + Cfg::Z_OFF + stage * Cfg::Z_BYTES + j * 128,
+                               zfrom + (static_cast<int64_t>(kb) * GPS + j) * p.Np, 128, wfull(stage));
+            }
+          }
+          __syncwarp();
+          if (++stage == Cfg::W_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    } else if (warp == Cfg::MMA_WARP) {
       // ------------------------------------------------------------------ MMA
       constexpr uint32_t kFmt = Cfg::F16 ? 0u : 1u;
       const uint32_t idesc = ptx::umma_idesc(kFmt, kFmt, 128, NMMA);
       constexpr int SPG = G / 16;                  // MMAs of one group
-      uint32_t blocks = 0, count = 0;              // (stage: that of the block's first 64 columns)
-      for (int item = first; item < items && ok; item += stride) {
-        for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks) {
-          const uint32_t buf = blocks % Cfg::A_BUFS;
-          if (!mbar_wait_warp(wc, afull(buf), blocks / Cfg::A_BUFS & 1u, kSiteSmemFull)) {
-            ok = false;
-            break;
-          }
-          const int stage1 = stage + 1 == Cfg::X_STAGES ? 0 : stage + 1;
-          const uint32_t phase1 = stage1 == 0 ? phase ^ 1u : phase;
+      uint32_t blocks = 0;
+      if constexpr (Cfg::HALVES == 1) {
+        // One block, B of the ring. All operands of the MMAs are constants beside two uniform base addresses: with addresses
+        // computed from a running index, each MMA of 32 columns took 49 cycles to issue (16 to execute).
+        auto multiply = [&](auto b_index) {
+          constexpr int B = decltype(b_index)::value;
+          const uint32_t x0 = ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + B * Cfg::XS_BYTES);
 #pragma unroll
-          for (int j = 0; j < GPS; ++j, ++count) {
-            if (j == 0 && !mbar_wait_warp(wc, xfull(stage), phase, kSiteSmemFull)) ok = false;
-            if ((j + 1) * G > 64 && j * G <= 64 && !mbar_wait_warp(wc, xfull(stage1), phase1, kSiteSmemFull)) ok = false;
-            if (!ok) break;
+          for (int u = 0; u < HPB; ++u) {
+            const int unit = (B * HPB + u) % Cfg::UNITS;
+            const uint32_t use = (blocks * HPB + u) / Cfg::UNITS;
+            const MbarPhase room = {dempty(unit), (use & 1u) ^ 1u, kSiteTmemEmpty};
+            const MbarPhase a = {afull(B % Cfg::A_BUFS), blocks / Cfg::A_BUFS & 1u, kSiteSmemFull};
+            const MbarPhase x = {xfull(B), blocks / Cfg::RING & 1u, kSiteSmemFull};
+            if (!(u == 0 ? mbar_wait_all_warp(wc, a, x, room) : mbar_wait_all_warp(wc, room))) return false;
+            ptx::tc_fence_after();
+            if (ptx::elect_one()) {
 #pragma unroll
-            for (int h = 0; h < Cfg::HALVES; ++h) {
-              const uint32_t d = Cfg::HALVES == 2 ? static_cast<uint32_t>(h) : count & 1u;
-              const uint32_t use = Cfg::HALVES == 2 ? count : count >> 1;
-              if (!mbar_wait_warp(wc, dempty(d), (use & 1u) ^ 1u, kSiteTmemEmpty)) {
-                ok = false;
-                break;
+              for (int s = u * GRAN * SPG; s < (u + 1) * GRAN * SPG; ++s) {
+                const uint32_t b_lo = x0 + (s / 4) * (TOK * 128 / 16) + 2u * (s % 4);
+                const uint32_t a_col = tmem + Cfg::A_COL + B % Cfg::A_BUFS * 64 + s * 8;
+                const uint32_t to = tmem + (unit * GRAN + s / SPG % GRAN) * NMMA;
+                if (s % SPG == 0) ptx::umma_ts_f16<false>(to, a_col, b_lo, idesc);
+                else ptx::umma_ts_f16<true>(to, a_col, b_lo, idesc);
               }
-              ptx::tc_fence_after();
-              if (ptx::elect_one()) {
-#pragma unroll
-                for (int s = j * SPG; s < (j + 1) * SPG; ++s) {
-                  const uint32_t xs = base + Cfg::X_OFF + (s < 4 ? stage : stage1) * Cfg::XS_BYTES + h * NMMA * 128;
-                  ptx::umma_ts_f16(tmem + d * NMMA, tmem + Cfg::A_COL + buf * 64 + s * 8,
-                                   ptx::umma_desc_k_sw128(xs) + 2u * (s % 4), idesc, s != j * SPG ? 1u : 0u);
-                }
-                ptx::umma_commit(dfull(d));
-                if (h == Cfg::HALVES - 1) {
-                  if (j * G < 64 && (j + 1) * G >= 64) ptx::umma_commit(xempty(stage));
-                  if (j == GPS - 1) {
-                    ptx::umma_commit(xempty(stage1));
-                    ptx::umma_commit(aempty(buf));
+              ptx::umma_commit(dfull(B * HPB + u));
+            }
+            __syncwarp();
+          }
+          return true;
+        };
+        for (int item = first; item < items && ok; item += stride) {
+          for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks) {
+            switch (blocks % Cfg::RING) {
+              case 0: ok = multiply(IntC<0>{}); break;
+              case 1: ok = multiply(IntC<1>{}); break;
+              case 2: ok = multiply(IntC<2>{}); break;
+              case 3: ok = multiply(IntC<3>{}); break;
+              default:
+                if constexpr (Cfg::RING == 8) {
+                  switch (blocks % Cfg::RING) {
+                    case 4: ok = multiply(IntC<4>{}); break;
+                    case 5: ok = multiply(IntC<5>{}); break;
+                    case 6: ok = multiply(IntC<6>{}); break;
+                    default: ok = multiply(IntC<7>{}); break;
                   }
                 }
-              }
-              __syncwarp();
             }
-            if (!ok) break;
           }
-          stage = stage1 + 1 == Cfg::X_STAGES ? 0 : stage1 + 1;
-          phase = stage == 0 ? phase1 ^ 1u : phase1;
+        }
+      } else {
+        // (stage: that of the block's first 64 columns)
+        uint32_t use[2] = {0, 0};                // of the two accumulators
+        for (int item = first; item < items && ok; item += stride) {
+          const Item it = item_of(item);
+          // a tile that ends early is multiplied as far as it goes, in steps of 16 rows
+          const int live = __shfl_sync(0xffffffffu, min(it.last - it.row, TOK), 0);
+          const int halves = live > NMMA ? 2 : 1;
+          const uint32_t idesc0 = ptx::umma_idesc(kFmt, kFmt, 128, min((live + 15) & ~15, NMMA));
+          const uint32_t idesc1 = ptx::umma_idesc(kFmt, kFmt, 128, max(min((live + 15 - NMMA) & ~15, NMMA), 16));
+          for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks) {
+            const uint32_t buf = blocks % Cfg::A_BUFS;
+            const int stage1 = stage + 1 == Cfg::X_STAGES ? 0 : stage + 1;
+            const uint32_t phase1 = stage1 == 0 ? phase ^ 1u : phase;
+            const uint32_t x0 = ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage * Cfg::XS_BYTES);
+            const uint32_t x1 = ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage1 * Cfg::XS_BYTES);
+            const uint32_t a_col = tmem + Cfg::A_COL + buf * 64;
+            const MbarPhase a = {afull(buf), blocks / Cfg::A_BUFS & 1u, kSiteSmemFull};
+            const MbarPhase xa = {xfull(stage), phase, kSiteSmemFull}, xb = {xfull(stage1), phase1, kSiteSmemFull};
+#pragma unroll
+            for (int j = 0; j < GPS; ++j) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (h == halves) break;
+                const MbarPhase room = {dempty(h), (use[h] & 1u) ^ 1u, kSiteTmemEmpty};
+                ++use[h];
+                if (h == 0 && j == 0) ok = GPS == 1 ? mbar_wait_all_warp(wc, a, xa, xb, room) : mbar_wait_all_warp(wc, a, xa, room);
+                else ok = h == 0 && j * G == 64 ? mbar_wait_all_warp(wc, xb, room) : mbar_wait_all_warp(wc, room);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                if (ptx::elect_one()) {
+#pragma unroll
+                  for (int s = j * SPG; s < (j + 1) * SPG; ++s) {
+                    const uint32_t b_lo = (s < 4 ? x0 : x1) + h * (NMMA * 128 / 16) + 2u * (s % 4);
+                    const uint32_t shape = h == 0 ? idesc0 : idesc1;
+                    if (s == j * SPG) ptx::umma_ts_f16<false>(tmem + h * NMMA, a_col + s * 8, b_lo, shape);
+                    else ptx::umma_ts_f16<true>(tmem + h * NMMA, a_col + s * 8, b_lo, shape);
+                  }
+                  ptx::umma_commit(dfull(h));
+                  if (h == halves - 1) {
+                    if (j * G < 64 && (j + 1) * G >= 64) ptx::umma_commit(xempty(stage));
+                    if (j == GPS - 1) {
+                      ptx::umma_commit(xempty(stage1));
+                      ptx::umma_commit(aempty(buf));
+                    }
+                  }
+                }
+                __syncwarp();
+              }
+              if (!ok) break;
+            }
+            stage = stage1 + 1 == Cfg::X_STAGES ? 0 : stage1 + 1;
+            phase = stage == 0 ? phase1 ^ 1u : phase1;
+          }
         }
       }
     }
     drain();
     if (S > 1) ptx::cluster_sync();
     else __syncthreads();
-    if (warp == 13) {
+    if (warp == Cfg::MMA_WARP) {
       ptx::tc_fence_after();
-      ptx::tmem_dealloc<1>(tmem, 512);
+      ptx::tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
     }
     __syncwarp();
     if (S > 1) ptx::cluster_sync();

@@ -116,6 +116,21 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// (without suspending the thread: cheaper where the phase is expected to be complete)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // ----------------------------------------------------------------------------------------
 // fences
 // ----------------------------------------------------------------------------------------
@@ -281,6 +296,11 @@ __device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const void* gsrc,
                "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(src_size)
                : "memory");
 }
+__device__ __forceinline__ void cp_async_8(uint32_t smem_dst, const void* gsrc, uint32_t src_size) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_dst),
+               "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(src_size)
+               : "memory");
+}
 __device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* gsrc) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(gsrc)) : "memory");
 }
@@ -412,13 +432,16 @@ __device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_
         : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem], kind::f16: row r of A in lane r, two elements along K per column.
-__device__ __forceinline__ void umma_ts_f16(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16: row r of A in lane r, two elements along K per column. B as for
+// umma_desc_k_sw128, whose upper half is constant: `b_lo` is the lower half, so that stepping along K is one 32-bit addition.
+__device__ __forceinline__ uint32_t umma_desc_k_sw128_lo(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
+template <bool ACC>
+__device__ __forceinline__ void umma_ts_f16(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc) {
+  constexpr uint32_t b_hi = (1024u >> 4) | 1u << 14 | 2u << 29;
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "n"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0)
       : "memory");
 }
 
@@ -482,6 +505,26 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 }
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// The same, naming the registers: nothing that uses them can move above the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]) : : "memory");
 }
 
 // ----------------------------------------------------------------------------------------
@@ -572,6 +615,13 @@ __device__ __forceinline__ ulonglong2 ld_shared_v2_b64(uint32_t saddr) {
   ulonglong2 v;
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(saddr));
   return v;
+}
+
+__device__ __forceinline__ void ld_shared_v4(uint32_t saddr, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(saddr));
+}
+__device__ __forceinline__ void ld_shared_v2(uint32_t saddr, uint32_t (&v)[2]) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(saddr));
 }
 
 // 16 bytes of shared memory of any CTA of the cluster (shared::cluster address, see mapa_u32)
@@ -701,6 +751,19 @@ __device__ __forceinline__ bool mbar_wait(const WaitCtx& w, uint32_t bar, uint32
 __device__ __forceinline__ bool mbar_wait_warp(const WaitCtx& w, uint32_t bar, uint32_t parity, uint32_t site) {
   if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(w, bar, parity, site));
+}
+
+// The phases that a warp needs before it goes on, by all its (converged) lanes. A wait that finds its phase complete still
+// costs a warp about 110 cycles, most of them between the answer, the vote and the branch; the tests of several phases overlap
+// and share the rest (three waits one after the other: 320 cycles).
+struct MbarPhase {
+  uint32_t bar, parity, site;
+};
+template <class... Phases>
+__device__ __forceinline__ bool mbar_wait_all_warp(const WaitCtx& w, const Phases&... ph) {
+  const bool ready = (static_cast<int>(ptx::mbar_test(ph.bar, ph.parity)) & ...) != 0;
+  if (__all_sync(0xffffffffu, ready)) return true;
+  return (mbar_wait_warp(w, ph.bar, ph.parity, ph.site) && ...);
 }
 
 // Wait until *flag >= expected (system-scope acquire; flags only ever grow). One thread.
