@@ -101,12 +101,27 @@ __global__ void __launch_bounds__(kGatedThreads) gated_kernel(const GatedParams 
     const P* gate = reinterpret_cast<const P*>(static_cast<const T*>(p.gate) + row * p.gate_stride);
     const P* up = reinterpret_cast<const P*>(static_cast<const T*>(p.up) + row * p.up_stride);
     const float r = p.row_weight != nullptr ? p.row_weight[row] : 1.f;
-    for (int c = t; c < chunks; c += p.tpr) {
-      const P g = gate[c], u = up[c];
-      P y;
+    // (narrow pieces: several at a time, all loads before the first use)
+    constexpr int U = V * sizeof(T) >= 16 ? 1 : V * sizeof(T) >= 8 ? 2 : 4;
+    for (int c0 = t; c0 < chunks; c0 += U * p.tpr) {
+      P g[U], u[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) y.v[j] = from_f32<T>(r * (act<T, ACT>(to_f32(g.v[j])) * to_f32(u.v[j])));
-      out[c] = y;
+      for (int i = 0; i < U; ++i) {
+        const int c = c0 + i * p.tpr;
+        if (U == 1 || c < chunks) {
+          g[i] = gate[c];
+          u[i] = up[c];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int c = c0 + i * p.tpr;
+        if (U > 1 && c >= chunks) break;
+        P y;
+#pragma unroll
+        for (int j = 0; j < V; ++j) y.v[j] = from_f32<T>(r * (act<T, ACT>(to_f32(g[i].v[j])) * to_f32(u[i].v[j])));
+        out[c] = y;
+      }
     }
   }
 }
@@ -136,19 +151,34 @@ __global__ void __launch_bounds__(kGatedThreads) gated_bwd_kernel(const GatedPar
         const P* up = reinterpret_cast<const P*>(static_cast<const T*>(p.up) + row * p.up_stride);
         const P* grad = reinterpret_cast<const P*>(static_cast<const T*>(p.grad) + row * p.grad_stride);
         const float r = p.row_weight != nullptr ? p.row_weight[row] : 1.f;
-        for (int c = t; c < chunks; c += p.tpr) {
-          const P g = gate[c], u = up[c], d = grad[c];
-          P dg, du;
+        constexpr int U = V * sizeof(T) >= 16 ? 1 : V * sizeof(T) >= 8 ? 2 : 4;
+        for (int c0 = t; c0 < chunks; c0 += U * p.tpr) {
+          P g[U], u[U], d[U];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float uj = to_f32(u.v[j]), dj = to_f32(d.v[j]);
-            const float2 a = act_slope<T, ACT>(to_f32(g.v[j]));
-            sum += dj * (a.x * uj);
-            dg.v[j] = from_f32<T>(r * (dj * (uj * a.y)));
-            du.v[j] = from_f32<T>(r * (dj * a.x));
+          for (int i = 0; i < U; ++i) {
+            const int c = c0 + i * p.tpr;
+            if (U == 1 || c < chunks) {
+              g[i] = gate[c];
+              u[i] = up[c];
+              d[i] = grad[c];
+            }
           }
-          dgate[c] = dg;
-          dup[c] = du;
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const int c = c0 + i * p.tpr;
+            if (U > 1 && c >= chunks) break;
+            P dg, du;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float uj = to_f32(u[i].v[j]), dj = to_f32(d[i].v[j]);
+              const float2 a = act_slope<T, ACT>(to_f32(g[i].v[j]));
+              sum += dj * (a.x * uj);
+              dg.v[j] = from_f32<T>(r * (dj * (uj * a.y)));
+              du.v[j] = from_f32<T>(r * (dj * a.x));
+            }
+            dgate[c] = dg;
+            dup[c] = du;
+          }
         }
       }
     }
@@ -174,7 +204,8 @@ int launch_gated(GatedParams& p, bool backward, cudaStream_t stream) {
   int sms = 0, rc;
   if ((rc = device_sm_count(&sms))) return rc;
   p.tpr = 32;
-  while (p.tpr < kGatedThreads && p.tpr * V < p.cols) p.tpr *= 2;
+  constexpr int U = V * sizeof(T) >= 16 ? 1 : V * sizeof(T) >= 8 ? 2 : 4;
+  while (p.tpr < kGatedThreads && p.tpr * V * U < p.cols) p.tpr *= 2;
   const int rpb = kGatedThreads / p.tpr;
   int64_t grid = (p.rows + rpb - 1) / rpb;
   if (grid > sms * 32ll) grid = sms * 32ll;

@@ -15,6 +15,11 @@
 //
 // One warp per token; a lane holds PER consecutive experts, so that the lowest lane with the largest value holds the
 // lowest index, and a row is read in 16-byte pieces.
+//
+// The choice is exact: it is the one that scores in real numbers give. Without a bias experts are compared by their logits.
+// Otherwise scores are computed in 32 bits with a bound on their error, and a token two of whose candidates (or groups) next to
+// each other in the order are closer than that is decided again in 64 bits, by the warp that found it (about 3 tokens in a
+// thousand with normal logits over 256 experts).
 #include "../include/fluxb.h"
 #include "../runtime/host_common.h"
 #include "../sm100/ptx.cuh"
@@ -63,7 +68,16 @@ __device__ __forceinline__ double value_of(uint64_t key) {
   const uint64_t b = key >> 63 ? key ^ 0x8000000000000000ull : ~key;
   return __longlong_as_double(static_cast<int64_t>(b));
 }
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (isnan(v)) return 1u;
+  const int32_t b = __float_as_int(v + 0.f);
+  return static_cast<uint32_t>(b) ^ (static_cast<uint32_t>(b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
 // largest key of the warp
+__device__ __forceinline__ uint32_t warp_max(uint32_t key) { return __reduce_max_sync(kFull, key); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t key) {
   const uint32_t hi = static_cast<uint32_t>(key >> 32);
   const uint32_t top = __reduce_max_sync(kFull, hi);
@@ -87,6 +101,31 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// The arithmetic of a choice. 32 bits: errors of the scores, fast exponential and division included. exp is good to
+// 2^-21 + |x| 2^-23 relative, and both x s (1 - s) and x exp(-x) stay below 0.4, so two sigmoids differ by what they should to
+// 2^-19, two softmax values (whose sum adds its own error) to 2^-18; sums of two to twice that.
+template <typename F>
+struct Num;
+template <>
+struct Num<float> {
+  using Key = uint32_t;
+  static constexpr bool kChecked = true;
+  static __device__ __forceinline__ float sigmoid(float l) {
+    const float s = __fdividef(1.f, 1.f + __expf(fminf(-l, 80.f)));
+    return isnan(l) ? l : s;
+  }
+  static __device__ __forceinline__ float power(float l, float top) { return __expf(l - top); }
+};
+template <>
+struct Num<double> {
+  using Key = uint64_t;
+  static constexpr bool kChecked = false;
+  static __device__ __forceinline__ double sigmoid(float l) { return 1.0 / (1.0 + exp(-static_cast<double>(l))); }
+  static __device__ __forceinline__ double power(float l, float top) {
+    return exp(static_cast<double>(l) - static_cast<double>(top));
+  }
+};
+
 // This lane's PER logits of one row; -inf past the last expert.
 template <typename T, int PER>
 __device__ __forceinline__ void load_row(const RouteParams& p, int64_t token, int lane, float (&l)[PER]) {
@@ -109,113 +148,222 @@ __device__ __forceinline__ void load_row(const RouteParams& p, int64_t token, in
   }
 }
 
-// Takes the largest of the lanes' keys k times; the lane of the winner drops it. Lane j < k returns the j-th expert.
-template <int PER>
-__device__ __forceinline__ int take_best(uint64_t (&key)[PER], int k, int lane) {
+// Whether two values that follow each other in the order are too close to be sure of it.
+__device__ __forceinline__ bool uncertain(float v, float next, float tau) { return v - next <= tau + fabsf(v) * 0x1p-22f; }
+
+// The k largest of the lanes' keys, largest first; lane j < k returns the j-th expert. `tau` >= 0: also whether neighbours in the
+// order, the first one that is left among them, are uncertain.
+// The (k + 1)-th largest of the lanes' own maxima bounds from below what can be among the first k + 1: the few keys that reach
+// it are packed into the first lanes, which then count the larger ones. About 200 instructions; taking one key after the other
+// costs 16 + 6 PER each, so it is left for a few experts out of up to 128 (16384 tokens, 6 of 120, with the gradient: 18.4 us
+// against 20.5; 8192 tokens, 8 of 256: 21 against 16.5), and for rows where more than 32 keys reach the bound.
+template <typename K, int PER>
+__device__ __forceinline__ int take_best(const K (&key)[PER], int k, int lane, float tau, K* buf /* shared, 32 */, bool& close) {
   int mine = 0;
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = key[0];
+  if (PER > 4 || k > 8) {
+    K own = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) own = max(own, key[i]);
+    buf[lane] = own;
+    __syncwarp();
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const K other = buf[i];
+      rank += other > own || (other == own && i < lane) ? 1 : 0;
+    }
+    __syncwarp();
+    const unsigned at_k = __ballot_sync(kFull, rank == k);              // (none: k = 32)
+    const K bound = at_k ? __shfl_sync(kFull, own, __ffs(at_k) - 1) : K(0);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) count += key[i] >= bound && key[i] != 0 ? 1 : 0;
+    int end = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kFull, end, o);
+      if (lane >= o) end += v;
+    }
+    const int total = __shfl_sync(kFull, end, 31);
+    if (bound != 0 && total <= 32) {
+      int to = end - count, which = 0;
+      K value = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (key[i] >= bound && key[i] != 0) {
+          buf[to] = key[i];
+          reinterpret_cast<int*>(buf + 32)[to] = lane * PER + i;
+          ++to;
+        }
+      }
+      __syncwarp();
+      if (lane < total) {
+        value = buf[lane];
+        which = reinterpret_cast<int*>(buf + 32)[lane];
+      }
+      int place = 0;
+      for (int i = 0; i < total; ++i) {
+        const K other = buf[i];
+        place += other > value || (other == value && i < lane) ? 1 : 0;
+      }
+      __syncwarp();
+      if (lane < total) {
+        buf[place] = value;
+        reinterpret_cast<int*>(buf + 32)[place] = which;
+      }
+      __syncwarp();
+      mine = lane < total ? reinterpret_cast<int*>(buf + 32)[lane] : 0;
+      if (tau >= 0.f) {
+        const K v = lane < total ? buf[lane] : K(0), next = lane + 1 < total ? buf[lane + 1] : K(0);
+        // (nothing left: certain; NaN: for the other path to say)
+        const float a = static_cast<float>(value_of(v)), b = static_cast<float>(value_of(next));
+        if (lane < k && next != 0 && (next == 1 || uncertain(a, b, tau))) close = true;
+      }
+      __syncwarp();
+      return mine;
+    }
+  }
+  uint32_t taken = 0;
+  float before = INFINITY;
+#pragma unroll 1
+  for (int j = 0; j <= k; ++j) {
+    K best = 0;
     int at = 0;
 #pragma unroll
-    for (int i = 1; i < PER; ++i) {
-      if (key[i] > best) {
+    for (int i = 0; i < PER; ++i) {
+      if (!(taken >> i & 1u) && key[i] > best) {
         best = key[i];
         at = i;
       }
     }
-    const uint64_t top = warp_max(best);
+    const K top = warp_max(best);
+    if (tau >= 0.f) {
+      const float v = top > 1 ? static_cast<float>(value_of(top)) : -INFINITY;
+      if (top == 1 || (j > 0 && top != 0 && uncertain(before, v, tau))) close = true;
+      before = v;
+    }
+    if (j == k) break;
     const int winner = __ffs(__ballot_sync(kFull, best == top)) - 1;
     const int e = __shfl_sync(kFull, lane * PER + at, winner);
     if (lane == j) mine = e;
-    if (lane == winner) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i == at) key[i] = 0;
-    }
+    if (lane == winner) taken |= 1u << at;
   }
   return mine;
 }
 
-// The choice in 64 bits: scores, group scores and comparisons in double precision. Without a bias the scores have the
-// order of the logits, which are compared as they are (scores that round to the same number stay apart).
-template <int PER>
-__device__ __forceinline__ int choose64(const RouteParams& p, const float (&l)[PER], float row_max, int lane,
-                                        uint64_t* keys /* shared, [E], with groups */) {
+// The choice in F; `close` (float): some comparison may have come out wrong.
+template <typename F, int PER>
+__device__ __forceinline__ int choose(const RouteParams& p, const float (&l)[PER], float row_max, int lane,
+                                      typename Num<F>::Key* keys /* shared: [E] with groups, 48 without */, bool& close) {
+  using N = Num<F>;
+  using K = typename N::Key;
   const int e0 = lane * PER;
-  uint64_t key[PER];
+  const bool by_logit = p.bias == nullptr, sums = p.groups > 1 && p.group_top == 2;
+  const float tau = p.sigmoid ? 0x1p-19f : 0x1p-18f;
+  K key[PER], gkey[PER];               // experts, and for the groups' scores
 #pragma unroll
-  for (int i = 0; i < PER; ++i) key[i] = e0 + i < p.E ? key_of(static_cast<double>(l[i])) : 0ull;
-  if (p.bias != nullptr || (p.groups > 1 && p.group_top == 2)) {
-    double s[PER];
+  for (int i = 0; i < PER; ++i) gkey[i] = key[i] = e0 + i < p.E ? static_cast<K>(key_of(static_cast<F>(l[i]))) : K(0);
+  if (!by_logit || sums) {
+    F s[PER];
     if (p.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) s[i] = 1.0 / (1.0 + exp(-static_cast<double>(l[i])));
+      for (int i = 0; i < PER; ++i) s[i] = N::sigmoid(l[i]);
     } else {
-      double sum = 0.0;
+      F sum = 0;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        s[i] = row_max == -INFINITY ? (isnan(l[i]) ? NAN : 0.0) : exp(static_cast<double>(l[i]) - static_cast<double>(row_max));
+        s[i] = row_max == -INFINITY ? (isnan(l[i]) ? static_cast<F>(NAN) : F(0)) : N::power(l[i], row_max);
         sum += s[i];
       }
       sum = warp_sum(sum);
-      if (sum != 0.0) {
+      const F inv = sum == F(0) ? F(0) : F(1) / sum;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) s[i] /= sum;
-      }
+      for (int i = 0; i < PER; ++i) s[i] *= inv;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const bool in = e0 + i < p.E;
-      if (p.bias != nullptr && in) key[i] = key_of(s[i] + static_cast<double>(p.bias[e0 + i]));
-      if (p.groups > 1 && in) keys[e0 + i] = p.bias != nullptr ? key[i] : key_of(s[i]);
+      if (!by_logit && in) s[i] += static_cast<F>(p.bias[e0 + i]);
+      if (in) gkey[i] = key_of(s[i]);
+      if (!by_logit) key[i] = gkey[i];
     }
-  } else if (p.groups > 1) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (e0 + i < p.E) keys[e0 + i] = key[i];
   }
   if (p.groups > 1) {
-    const int size = p.E / p.groups;
-    __syncwarp();
-    uint64_t mine = 0;             // lane g: key of group g's score
-    for (int g = 0; g < p.groups; ++g) {
-      uint64_t a = 0, b = 0;       // the two largest of this lane's share
-      for (int i = lane; i < size; i += 32) {
-        const uint64_t x = keys[g * size + i];
-        if (x > a) {
-          b = a;
-          a = x;
-        } else if (x > b) {
-          b = x;
+    const int size = p.E / p.groups, span = size / PER;           // experts of a group; lanes, if it begins and ends with lanes
+    K mine = 0;                                                   // lane g: key of group g's score
+    const bool whole = size % PER == 0 && (span & (span - 1)) == 0;
+    if (whole) {
+      K a = 0, b = 0;                                             // the two largest of this lane, then of its group
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        b = max(b, min(a, gkey[i]));
+        a = max(a, gkey[i]);
+      }
+      for (int o = 1; o < span; o <<= 1) {
+        const K a2 = __shfl_xor_sync(kFull, a, o), b2 = __shfl_xor_sync(kFull, b, o);
+        b = max(min(a, a2), max(b, b2));
+        a = max(a, a2);
+      }
+      K total = a;
+      // (key 1 stands for NaN, which makes the sum the lowest too)
+      if (p.group_top == 2) total = b <= 1 ? K(1) : static_cast<K>(key_of(value_of(a) + value_of(b)));
+      mine = __shfl_sync(kFull, total, min(lane * span, 31));
+      if (lane >= p.groups) mine = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e0 + i < p.E) keys[e0 + i] = gkey[i];
+      __syncwarp();
+#pragma unroll 1
+      for (int g = 0; g < p.groups; ++g) {
+        K a = 0, b = 0;
+        for (int i = lane; i < size; i += 32) {
+          const K x = keys[g * size + i];
+          b = max(b, min(a, x));
+          a = max(a, x);
         }
+        const K first = warp_max(a);
+        K total = first;
+        if (p.group_top == 2) {
+          const int winner = __ffs(__ballot_sync(kFull, a == first)) - 1;
+          const K second = warp_max(lane == winner ? b : a);
+          total = second <= 1 ? K(1) : static_cast<K>(key_of(value_of(first) + value_of(second)));
+        }
+        if (lane == g) mine = total;
       }
-      const uint64_t first = warp_max(a);
-      uint64_t total = first;
-      if (p.group_top == 2) {
-        const int winner = __ffs(__ballot_sync(kFull, a == first)) - 1;
-        const uint64_t second = warp_max(lane == winner ? b : a);
-        // (key 1 stands for NaN, which makes the sum the lowest too)
-        total = first == 1 || second == 1 ? 1ull : key_of(value_of(first) + value_of(second));
-      }
-      if (lane == g) mine = total;
+      __syncwarp();
     }
     int rank = 0;
     for (int g = 0; g < p.groups; ++g) {
-      const uint64_t other = __shfl_sync(kFull, mine, g);
+      const K other = __shfl_sync(kFull, mine, g);
       rank += other > mine || (other == mine && g < lane) ? 1 : 0;
     }
-    const unsigned kept = __ballot_sync(kFull, lane < p.groups && rank < p.topk_groups);
+    const bool group = lane < p.groups;
+    const unsigned kept = __ballot_sync(kFull, group && rank < p.topk_groups);
+    if (N::kChecked && (!by_logit || sums) && p.topk_groups < p.groups) {
+      // the last group that stays and the first that goes
+      const K in = __shfl_sync(kFull, mine, __ffs(__ballot_sync(kFull, group && rank == p.topk_groups - 1)) - 1);
+      const K out = __shfl_sync(kFull, mine, __ffs(__ballot_sync(kFull, group && rank == p.topk_groups)) - 1);
+      const float v = static_cast<float>(value_of(in)), w = static_cast<float>(value_of(out));
+      if (in <= 1 || out <= 1 || !(v - w > 2.f * tau + fabsf(v) * 0x1p-21f)) close = true;
+    }
+    if (whole) {
+      const bool out = !(kept >> min(lane / span, 31) & 1u);
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (e0 + i < p.E && !(kept >> ((e0 + i) / size) & 1u)) key[i] = 0;
-    __syncwarp();
+      for (int i = 0; i < PER; ++i)
+        if (out) key[i] = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e0 + i < p.E && !(kept >> ((e0 + i) / size) & 1u)) key[i] = 0;
+    }
   }
-  return take_best<PER>(key, p.k, lane);
+  return take_best<K, PER>(key, p.k, lane, N::kChecked && !by_logit ? tau : -1.f, keys, close);
 }
 
 template <typename T, int PER>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
-  extern __shared__ uint64_t group_keys[];          // [warps][E], with groups only
+  extern __shared__ uint64_t key_space[];           // [warps][max(E, 48)]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
   if (token >= p.tokens) return;
@@ -225,7 +373,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
 #pragma unroll
   for (int i = 1; i < PER; ++i) top = fmaxf(top, l[i]);
   const float row_max = warp_max(top);
-  const int e = choose64<PER>(p, l, row_max, lane, group_keys + warp * p.E);
+  bool close = false;
+  uint64_t* const keys = key_space + warp * max(p.E, 48);
+  int e = choose<float, PER>(p, l, row_max, lane, reinterpret_cast<uint32_t*>(keys), close);
+  if (__any_sync(kFull, close)) e = choose<double, PER>(p, l, row_max, lane, keys, close);
 
   // weights: lane j holds the j-th expert
   const bool live = lane < p.k;
@@ -341,7 +492,7 @@ int launch_route(RouteParams& p, bool backward, cudaStream_t stream) {
   if (backward) {
     route_bwd_kernel<T, PER><<<static_cast<unsigned>(grid), kRouteWarps * 32, 0, stream>>>(p);
   } else {
-    const size_t smem = p.groups > 1 ? sizeof(uint64_t) * kRouteWarps * p.E : 0;
+    const size_t smem = sizeof(uint64_t) * kRouteWarps * (p.E > 48 ? p.E : 48);
     route_kernel<T, PER><<<static_cast<unsigned>(grid), kRouteWarps * 32, smem, stream>>>(p);
   }
   FLUXB_CUDA_OK(cudaGetLastError());

@@ -53,27 +53,34 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _args(gate, up, act, row_weight, num_rows) -> GatedArgs:
+def _args(gate, up, act, row_weight, num_rows, device) -> GatedArgs:
+    """``up`` None: both halves are in ``gate``."""
     a = GatedArgs()
-    a.gate, a.gate_stride, a.up, a.up_stride = gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0)
-    a.rows, a.cols = up.shape
+    rows, cols = gate.shape
+    a.gate, a.gate_stride = gate.data_ptr(), gate.stride(0)
+    if up is None:
+        cols //= 2
+        a.up, a.up_stride = gate.data_ptr() + cols * gate.element_size(), gate.stride(0)
+    else:
+        a.up, a.up_stride = up.data_ptr(), up.stride(0)
+    a.rows, a.cols = rows, cols
     a.dtype, a.act = dtype_code(gate.dtype), ACT[act]
     if row_weight is not None:
         a.row_weight = row_weight.data_ptr()
     if num_rows is not None:
         a.num_rows, a.num_rows_64 = num_rows.data_ptr(), int(num_rows.dtype == torch.int64)
-    a.stream = current_stream_ptr(gate.device)
+    a.stream = current_stream_ptr(device)
     return a
 
 
 def _forward(gate, up, act, row_weight, num_rows, out):
-    gate, up = _rows(gate), _rows(up)
-    fresh = out is None
+    gate, up = _rows(gate), None if up is None else _rows(up)
+    fresh, device = out is None, gate.device
     if fresh:
-        out = torch.empty(up.shape, dtype=gate.dtype, device=gate.device)
-    with device_guard(gate.device):
-        a = _args(gate, up, act, row_weight, num_rows)
-        a.out, a.out_stride, a.zero_rest = out.data_ptr(), out.stride(0), int(fresh)
+        out = gate.new_empty((gate.shape[0], gate.shape[1] // 2 if up is None else gate.shape[1]))
+    with device_guard(device):
+        a = _args(gate, up, act, row_weight, num_rows, device)
+        a.out, a.out_stride, a.zero_rest = out.data_ptr(), out.stride(0), fresh
         _native.check(_native.lib().fluxb_gated_act(ctypes.byref(a)), "fluxb_gated_act")
     return out
 
@@ -81,35 +88,30 @@ def _forward(gate, up, act, row_weight, num_rows, out):
 class _Gated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, row_weight, act, num_rows):
-        # (up None: gate holds both halves)
         ctx.save_for_backward(gate, up, row_weight, num_rows)
         ctx.act = act
-        cols = gate.shape[1] // 2
-        return _forward(gate if up is not None else gate[:, :cols], up if up is not None else gate[:, cols:], act,
-                        row_weight, num_rows, None)
+        return _forward(gate, up, act, row_weight, num_rows, None)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         gate, up, row_weight, num_rows = ctx.saved_tensors
-        grad = _rows(grad)
-        rows, cols = grad.shape
-        if up is None:
-            dboth = torch.empty((rows, 2 * cols), dtype=gate.dtype, device=gate.device)
-            dgate, dup = dboth[:, :cols], dboth[:, cols:]
-            g, u = _rows(gate[:, :cols]), _rows(gate[:, cols:])
-        else:
-            dgate = torch.empty((rows, cols), dtype=gate.dtype, device=gate.device)
-            dup = torch.empty((rows, cols), dtype=gate.dtype, device=gate.device)
-            g, u = _rows(gate), _rows(up)
+        grad, gate, up = _rows(grad), _rows(gate), None if up is None else _rows(up)
+        device = gate.device
+        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=device)
+        dup = torch.empty(up.shape, dtype=gate.dtype, device=device) if up is not None else None
         drow = torch.empty_like(row_weight) if row_weight is not None and ctx.needs_input_grad[2] else None
-        with device_guard(gate.device):
-            a = _args(g, u, ctx.act, row_weight, num_rows)
+        with device_guard(device):
+            a = _args(gate, up, ctx.act, row_weight, num_rows, device)
             a.grad, a.grad_stride = grad.data_ptr(), grad.stride(0)
-            a.dgate, a.dgate_stride, a.dup, a.dup_stride = dgate.data_ptr(), dgate.stride(0), dup.data_ptr(), dup.stride(0)
+            a.dgate, a.dgate_stride = dgate.data_ptr(), dgate.stride(0)
+            if up is None:
+                a.dup, a.dup_stride = dgate.data_ptr() + a.cols * gate.element_size(), dgate.stride(0)
+            else:
+                a.dup, a.dup_stride = dup.data_ptr(), dup.stride(0)
             a.drow = drow.data_ptr() if drow is not None else None
             _native.check(_native.lib().fluxb_gated_act_bwd(ctypes.byref(a)), "fluxb_gated_act_bwd")
-        return (dboth if up is None else dgate), (dup if up is not None else None), drow, None, None
+        return dgate, dup, drow, None, None
 
 
 def gated_act(gate: torch.Tensor, up: Optional[torch.Tensor] = None, act: str = "silu",
@@ -139,7 +141,8 @@ def gated_act(gate: torch.Tensor, up: Optional[torch.Tensor] = None, act: str = 
     if num_rows is not None and (num_rows.numel() != 1 or num_rows.dtype not in (torch.int32, torch.int64)
                                  or num_rows.device != gate.device):
         raise ValueError("num_rows must be one int32 or int64 on the device of gate")
-    grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (gate, up, row_weight))
+    grads = torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)
+                                         or (row_weight is not None and row_weight.requires_grad))
     if out is not None:
         if grads:
             raise ValueError("out cannot be used where gradients are recorded")
@@ -158,6 +161,4 @@ def gated_act(gate: torch.Tensor, up: Optional[torch.Tensor] = None, act: str = 
         row_weight = row_weight.contiguous()
     if grads:
         return _Gated.apply(gate, up, row_weight, act, num_rows)
-    if up is None:
-        gate, up = gate[:, :cols], gate[:, cols:]
     return _forward(gate, up, act, row_weight, num_rows, out)

@@ -92,26 +92,24 @@ def moe_route_torch(logits: torch.Tensor, topk: int, score_func: str = "softmax"
     return experts.to(torch.int32), (w * scale).float()
 
 
-def _args(logits, experts, weights, cfg) -> RouteArgs:
-    topk, score, _, groups, topk_groups, group_top, renorm, scale = cfg
+def _args(logits, experts, weights, cfg, device) -> RouteArgs:
     a = RouteArgs()
     a.logits, a.row_stride, a.dtype = logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype)
     a.experts, a.weights = experts.data_ptr(), weights.data_ptr()
     a.tokens, a.num_experts = logits.shape
-    a.topk, a.num_groups, a.topk_groups, a.group_top = topk, groups, topk_groups, group_top
-    a.score, a.renormalize, a.scale = _SCORES[score], int(renorm), scale
-    a.stream = current_stream_ptr(logits.device)
+    a.topk, a.score, bias, a.num_groups, a.topk_groups, a.group_top, a.renormalize, a.scale = cfg
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    a.stream = current_stream_ptr(device)
     return a
 
 
 def _forward(logits, cfg):
     x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
-    experts = torch.empty((x.shape[0], cfg[0]), dtype=torch.int32, device=x.device)
-    weights = torch.empty((x.shape[0], cfg[0]), dtype=torch.float32, device=x.device)
-    with device_guard(x.device):
-        a = _args(x, experts, weights, cfg)
-        if cfg[2] is not None:
-            a.bias = cfg[2].data_ptr()
+    device, shape = x.device, (x.shape[0], cfg[0])
+    experts, weights = x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
+    with device_guard(device):
+        a = _args(x, experts, weights, cfg, device)
         _native.check(_native.lib().fluxb_moe_route(ctypes.byref(a)), "fluxb_moe_route")
     return x, experts, weights
 
@@ -132,7 +130,7 @@ class _Route(torch.autograd.Function):
         grad = grad.to(torch.float32).contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         with device_guard(x.device):
-            a = _args(x, experts, weights, ctx.cfg)
+            a = _args(x, experts, weights, ctx.cfg, x.device)
             a.grad, a.dlogits = grad.data_ptr(), dx.data_ptr()
             _native.check(_native.lib().fluxb_moe_route_bwd(ctypes.byref(a)), "fluxb_moe_route_bwd")
         return dx, None
@@ -178,7 +176,7 @@ def moe_route(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias
         topk_groups = group_top = 1
     if not logits.is_cuda:
         return moe_route_torch(logits, topk, score_func, bias, num_groups, topk_groups, group_top, renormalize, scale)
-    cfg = (topk, score_func, bias, num_groups, topk_groups, group_top, bool(renormalize), scale)
+    cfg = (topk, _SCORES[score_func], bias, num_groups, topk_groups, group_top, bool(renormalize), scale)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Route.apply(logits, cfg)
     return _forward(logits, cfg)[1:]
