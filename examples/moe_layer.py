@@ -2,6 +2,8 @@
 all GPUs (reference: examples/moe_flux_only.py).
 
     ./launch.sh examples/moe_layer.py --tokens-per-rank 8192 --experts 64 --topk 8
+
+``--int4`` (one rank) serves the same layer with 4-bit expert weights.
 """
 import argparse
 import os
@@ -12,7 +14,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))  # run from a checkout
 
 import tempname_new_b200 as flux
-from tempname_new_b200.testing import gate_func, initialize_distributed, run_perf
+from tempname_new_b200.testing import initialize_distributed, run_perf
 
 ap = argparse.ArgumentParser()
 ap.add_argument("--tokens-per-rank", type=int, default=2048)
@@ -20,6 +22,7 @@ ap.add_argument("--hidden", type=int, default=4096)
 ap.add_argument("--ffn", type=int, default=1536)
 ap.add_argument("--experts", type=int, default=64)
 ap.add_argument("--topk", type=int, default=8)
+ap.add_argument("--int4", action="store_true", help="4-bit expert weights (one rank)")
 args = ap.parse_args()
 
 pg = initialize_distributed()
@@ -42,7 +45,7 @@ x = torch.randn(args.tokens_per_rank, H, device=DEV).to(DT)
 
 def layer():
     # routing needs every rank's choices: gather the (small) router outputs
-    chosen, gate = gate_func(x, router, topk)
+    chosen, gate = flux.moe_route(x.float() @ router.float().t(), topk)
     all_chosen = torch.empty(tokens, topk, dtype=torch.int32, device=DEV)
     all_gate = torch.empty(tokens, topk, dtype=torch.float32, device=DEV)
     torch.distributed.all_gather_into_tensor(all_chosen, chosen.contiguous(), group=pg)
@@ -52,11 +55,28 @@ def layer():
     rows = int(hi - lo)                                        # the only host sync: sizing the buffers
     h = torch.empty(rows, 2 * F, dtype=DT, device=DEV)
     layer0.forward(x, w_gate_up, splits, scatter, outputs_buf=h)
-    act = torch.nn.functional.silu(h[:, :F].float()).mul_(h[:, F:].float()).to(DT)
+    act = flux.gated_act(h)
     row_gate = all_gate.reshape(-1)[gather.long() * topk + tki.long()][int(lo):int(hi)].contiguous()
     return layer1.forward_gather_rs(act, w_down, splits, scatter.reshape(-1), output_vec_scale=row_gate)
 
 
+def layer_int4():
+    # every row goes through both products with its own expert's weights; nothing is read back to size a buffer
+    chosen, gate = flux.moe_route(x.float() @ router.float().t(), topk)
+    splits, offsets, scatter, gather, tki = flux.moe_index_build(chosen, E)
+    row_gate = gate.reshape(-1)[gather.long() * topk + tki.long()]
+    h = gate_up4.forward(x[gather.long()], splits)
+    act = flux.gated_act(h, row_weight=row_gate, num_rows=offsets[-1:])
+    return flux.topk_scatter_reduce(down4.forward(act, splits), scatter.reshape(-1), topk)
+
+
+if args.int4:
+    if world != 1:
+        raise SystemExit("--int4 runs on one rank")
+    group = 128 if H % 128 == 0 and F % 128 == 0 else 32
+    gate_up4 = flux.Int4GemmGrouped(*flux.quantize_int4(w_gate_up, group))
+    down4 = flux.Int4GemmGrouped(*flux.quantize_int4(w_down, group))
+    layer = layer_int4
 y, ms = run_perf("moe_layer", 2, 5, layer)
 if rank == 0:
     print(f"MoE layer E={E} top{topk} hidden {H} ffn {F}, {args.tokens_per_rank} tokens/rank on {world} GPUs: "

@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
+from ..parallel.symm import FluxTimeoutError
 from ._dense import current_stream_ptr, device_guard, dtype_code
 
 _VP = ctypes.c_void_p
@@ -135,9 +136,16 @@ class _Int4Weights:
         a.packed, a.scales_out = self.packed.data_ptr(), self.packed_scales.data_ptr()
         a.zeros_out = self.packed_zeros.data_ptr() if zeros is not None else None
         a.experts, a.N, a.K, a.group = self.E, self.N, self.K, self.group
+        self._status = torch.zeros(4, dtype=torch.int32, device=self.device)
         with device_guard(self.device):
             a.stream = current_stream_ptr(self.device)
             _native.check(_native.lib().fluxb_int4_layout(ctypes.byref(a)), "fluxb_int4_layout")
+
+    def check_status(self) -> None:
+        """Raises if a wait inside a launch so far ran out of time (its results are then not to be used)."""
+        if self.device.type == "cuda" and self._status.tolist()[0] != 0:
+            self._status.zero_()
+            raise FluxTimeoutError("product with 4-bit weights: a wait inside the kernel timed out")
 
     # ------------------------------------------------------------------------------
     def _check_input(self, x, output_buf):
@@ -170,7 +178,7 @@ class _Int4Weights:
         if splits is not None:
             a.splits = splits.data_ptr()
         a.experts, a.N, a.K, a.group = self.E, self.N, self.K, self.group
-        a.dtype, a.scale_dtype = dtype_code(x.dtype), dtype_code(self.scale_dtype)
+        a.dtype, a.scale_dtype, a.status = dtype_code(x.dtype), dtype_code(self.scale_dtype), self._status.data_ptr()
         with device_guard(x.device):
             a.stream = current_stream_ptr(x.device)
             _native.check(_native.lib().fluxb_int4_gemm(ctypes.byref(a)), "fluxb_int4_gemm")

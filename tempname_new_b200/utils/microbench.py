@@ -250,6 +250,66 @@ def cmd_small(a):
                       "gbs": x.numel() * 4 / ms / 1e6, "frac_of_hbm_peak": x.numel() * 4 / ms / 1e6 / pk, "peak": src}))
 
 
+def cmd_route(a):
+    """Choice of experts from router logits (``--train``: and the gradient of the weights)."""
+    import tempname_new_b200 as flux
+    dev = torch.device("cuda")
+    x = torch.randn(a.tokens, a.experts, device=dev).requires_grad_(a.train)
+    bias = torch.randn(a.experts, device=dev) * 0.05 if a.bias else None
+    gw = torch.randn(a.tokens, a.topk, device=dev)
+
+    def fn():
+        w = flux.moe_route(x, a.topk, a.score, bias, a.groups, a.topk_groups, min(2, a.experts // a.groups))[1]
+        if a.train:
+            torch.autograd.grad(w, x, gw)
+    ms = timed(fn, a.iters, a.warmup, not a.no_flush)
+    nbytes = a.tokens * (a.experts * 4 * (3 if a.train else 1) + a.topk * (16 if a.train else 8))
+    _, pk, src = peaks()
+    print(json.dumps({"op": "moe_route", "tokens": a.tokens, "experts": a.experts, "topk": a.topk, "score": a.score,
+                      "train": a.train, "ms": ms, "gbs": nbytes / ms / 1e6, "frac_of_hbm_peak": nbytes / ms / 1e6 / pk,
+                      "peak": src}))
+
+
+def cmd_gated(a):
+    """Gated activation of [rows, 2 * cols] (``--train``: and its gradient)."""
+    import tempname_new_b200 as flux
+    dev = torch.device("cuda")
+    x = torch.randn(a.rows, 2 * a.cols, device=dev).bfloat16().requires_grad_(a.train)
+    dy = torch.randn(a.rows, a.cols, device=dev).bfloat16()
+
+    def fn():
+        y = flux.gated_act(x, act=a.act)
+        if a.train:
+            torch.autograd.grad(y, x, dy)
+    ms = timed(fn, a.iters, a.warmup, not a.no_flush)
+    nbytes = a.rows * a.cols * 2 * (8 if a.train else 3)
+    _, pk, src = peaks()
+    print(json.dumps({"op": "gated_act", "rows": a.rows, "cols": a.cols, "act": a.act, "train": a.train, "ms": ms,
+                      "gbs": nbytes / ms / 1e6, "frac_of_hbm_peak": nbytes / ms / 1e6 / pk, "peak": src}))
+
+
+def cmd_int4(a):
+    """Product with 4-bit weights, dense or (``--experts``) over equally long runs of rows."""
+    import tempname_new_b200 as flux
+    dev, lead = torch.device("cuda"), (a.experts,) if a.experts else ()
+    q = torch.randint(0, 256, (*lead, a.n, a.k // 2), device=dev, dtype=torch.uint8)
+    s = (torch.rand(*lead, a.n, a.k // a.group, device=dev) * 0.02).bfloat16()
+    z = torch.randint(4, 12, s.shape, device=dev, dtype=torch.uint8) if a.zeros else None
+    x = torch.randn(a.m, a.k, device=dev).bfloat16()
+    if a.experts:
+        op, splits = flux.Int4GemmGrouped(q, s, z), torch.full((a.experts,), a.m // a.experts, device=dev, dtype=torch.int32)
+        fn = lambda: op.forward(x, splits)  # noqa: E731
+    else:
+        op = flux.Int4Gemm(q, s, z)
+        fn = lambda: op.forward(x)  # noqa: E731
+    ms = timed(fn, a.iters, a.warmup, not a.no_flush)
+    nbytes = q.numel() + s.numel() * (3 if a.zeros else 2) + 2 * a.m * (a.n + a.k)
+    tf, (ptf, pk, src) = 2.0 * a.m * a.n * a.k / ms / 1e9, peaks()
+    print(json.dumps({"op": "int4", "m": a.m, "n": a.n, "k": a.k, "group": a.group, "experts": a.experts, "ms": ms,
+                      "gbs": nbytes / ms / 1e6, "frac_of_hbm_peak": nbytes / ms / 1e6 / pk, "tflops": tf,
+                      "frac_of_bf16_peak": tf / ptf, "peak": src}))
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(prog="microbench")
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -308,7 +368,31 @@ def main(argv=None):
     sm = sub.add_parser("small")
     sm.add_argument("--elems", type=int, default=1 << 26)
     sm.set_defaults(fn=cmd_small)
-    for p in (g, q, b, gg, u, c, sm, m1):
+    rt = sub.add_parser("route")
+    rt.add_argument("--tokens", type=int, default=8192)
+    rt.add_argument("--experts", type=int, default=256)
+    rt.add_argument("--topk", type=int, default=8)
+    rt.add_argument("--groups", type=int, default=1)
+    rt.add_argument("--topk-groups", type=int, default=1)
+    rt.add_argument("--score", default="softmax", choices=["softmax", "sigmoid"])
+    rt.add_argument("--bias", action="store_true")
+    rt.add_argument("--train", action="store_true")
+    rt.set_defaults(fn=cmd_route)
+    ga = sub.add_parser("gated")
+    ga.add_argument("--rows", type=int, default=32768)
+    ga.add_argument("--cols", type=int, default=2048)
+    ga.add_argument("--act", default="silu", choices=["silu", "gelu", "relu"])
+    ga.add_argument("--train", action="store_true")
+    ga.set_defaults(fn=cmd_gated)
+    i4 = sub.add_parser("int4")
+    i4.add_argument("--m", type=int, default=1)
+    i4.add_argument("--n", type=int, default=16384)
+    i4.add_argument("--k", type=int, default=4096)
+    i4.add_argument("--group", type=int, default=128)
+    i4.add_argument("--experts", type=int, default=0)
+    i4.add_argument("--zeros", action="store_true")
+    i4.set_defaults(fn=cmd_int4)
+    for p in (g, q, b, gg, u, c, sm, m1, rt, ga, i4):
         p.add_argument("--iters", type=int, default=10)
         p.add_argument("--warmup", type=int, default=3)
         p.add_argument("--no-flush", action="store_true")

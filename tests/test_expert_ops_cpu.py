@@ -214,3 +214,15 @@ def test_native_argument_checks(lib_built):
         assert lib.fluxb_int4_gemm(ctypes.byref(d)) == 1, bad
     for f in (lib.fluxb_moe_route, lib.fluxb_gated_act, lib.fluxb_int4_layout, lib.fluxb_int4_gemm):
         assert f(None) == 1
+
+
+def test_example_with_int4_weights():
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT, free_port
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "1", "--master-addr", "127.0.0.1",
+           "--master-port", str(free_port()), os.path.join(ROOT, "examples", "moe_layer.py"), "--tokens-per-rank", "16",
+           "--hidden", "64", "--ffn", "32", "--experts", "4", "--topk", "2", "--int4"]
+    r = subprocess.run(cmd, cwd=ROOT, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""), capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "MoE layer E=4 top2" in r.stdout, r.stdout[-1500:] + r.stderr[-3000:]

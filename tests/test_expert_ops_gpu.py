@@ -464,3 +464,16 @@ def test_expert_layer_together(dev, flux):
     oracle.assert_within(act, ref, bound)
     ref = y[scatter.long()].double()
     oracle.assert_within(out, ref.sum(1), ref.abs().sum(1) * 4 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("args,op", [
+    (["route", "--tokens", "500", "--experts", "64", "--groups", "4", "--topk-groups", "2", "--bias", "--train"], "moe_route"),
+    (["gated", "--rows", "300", "--cols", "128", "--train"], "gated_act"),
+    (["int4", "--m", "5", "--n", "256", "--k", "512", "--zeros"], "int4"),
+    (["int4", "--m", "64", "--n", "256", "--k", "512", "--group", "32", "--experts", "8"], "int4")])
+def test_microbench_commands(dev, args, op, capsys):
+    import json
+    from tempname_new_b200.utils import microbench
+    microbench.main(args + ["--iters", "2", "--warmup", "1", "--no-flush"])
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert line["op"] == op and line["ms"] > 0
