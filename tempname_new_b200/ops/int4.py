@@ -140,6 +140,12 @@ class _Int4Weights:
         with device_guard(self.device):
             a.stream = current_stream_ptr(self.device)
             _native.check(_native.lib().fluxb_int4_layout(ctypes.byref(a)), "fluxb_int4_layout")
+        a = self._args = Int4GemmArgs()                # what every call has in common
+        a.packed, a.scales = self.packed.data_ptr(), self.packed_scales.data_ptr()
+        if self.packed_zeros is not None:
+            a.zeros = self.packed_zeros.data_ptr()
+        a.experts, a.N, a.K, a.group = self.E, self.N, self.K, self.group
+        a.scale_dtype, a.status = dtype_code(self.scale_dtype), self._status.data_ptr()
 
     def check_status(self) -> None:
         """Raises if a wait inside a launch so far ran out of time (its results are then not to be used)."""
@@ -149,38 +155,38 @@ class _Int4Weights:
 
     # ------------------------------------------------------------------------------
     def _check_input(self, x, output_buf):
-        if x.dim() != 2 or x.shape[1] != self.K:
-            raise ValueError(f"input must be [rows, {self.K}], got {tuple(x.shape)}")
-        if x.dtype not in _HALF and (x.is_cuda or x.dtype != torch.float32):
-            raise TypeError(f"input must be bfloat16 or float16, got {x.dtype}")
+        shape, dtype = x.shape, x.dtype
+        if len(shape) != 2 or shape[1] != self.K:
+            raise ValueError(f"input must be [rows, {self.K}], got {tuple(shape)}")
+        if dtype not in _HALF and (x.is_cuda or dtype != torch.float32):
+            raise TypeError(f"input must be bfloat16 or float16, got {dtype}")
         if x.device != self.device:
             raise ValueError(f"input is on {x.device}, the weights on {self.device}")
-        if torch.is_grad_enabled() and x.requires_grad:
+        if x.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("products with 4-bit weights have no backward; call them under torch.no_grad()")
-        if output_buf is not None and (output_buf.shape != (x.shape[0], self.N) or output_buf.dtype != x.dtype
-                                       or output_buf.device != x.device or (self.N > 1 and output_buf.stride(1) != 1)):
+        if output_buf is not None and (output_buf.shape != (shape[0], self.N) or output_buf.dtype != dtype
+                                       or output_buf.device != self.device or (self.N > 1 and output_buf.stride(1) != 1)):
             raise ValueError("output_buf must be [rows, N] of the input's type, on its device, with contiguous rows")
 
     def _launch(self, x, bias, splits, output_buf):
-        out = output_buf if output_buf is not None else torch.empty((x.shape[0], self.N), dtype=x.dtype, device=x.device)
-        if x.shape[0] > 1 and (x.stride(1) != 1 or x.stride(0) % 8):
-            x = x.contiguous()
-        if x.stride(1) != 1 or x.data_ptr() % 16:
+        rows = x.shape[0]
+        out = output_buf if output_buf is not None else x.new_empty((rows, self.N))
+        ldx, inner = x.stride()
+        if rows == 1:
+            ldx = self.K
+        ptr = x.data_ptr()
+        if inner != 1 or ldx % 8 or ptr % 16:          # (the kernels read rows in 16-byte pieces)
             x = x.clone(memory_format=torch.contiguous_format)
-        a = Int4GemmArgs()
-        a.x, a.out = x.data_ptr(), out.data_ptr()
-        a.M, a.ldx, a.ldo = x.shape[0], x.stride(0) if x.shape[0] > 1 else self.K, out.stride(0)
-        a.packed, a.scales = self.packed.data_ptr(), self.packed_scales.data_ptr()
-        if self.packed_zeros is not None:
-            a.zeros = self.packed_zeros.data_ptr()
+            ldx, ptr = self.K, x.data_ptr()
+        a = Int4GemmArgs.from_buffer_copy(self._args)  # (a copy: calls may come from several threads)
+        a.x, a.out, a.M, a.ldx, a.ldo = ptr, out.data_ptr(), rows, ldx, out.stride(0)
         if bias is not None:
             a.bias = bias.data_ptr()
         if splits is not None:
             a.splits = splits.data_ptr()
-        a.experts, a.N, a.K, a.group = self.E, self.N, self.K, self.group
-        a.dtype, a.scale_dtype, a.status = dtype_code(x.dtype), dtype_code(self.scale_dtype), self._status.data_ptr()
-        with device_guard(x.device):
-            a.stream = current_stream_ptr(x.device)
+        a.dtype = dtype_code(x.dtype)
+        with device_guard(self.device):
+            a.stream = current_stream_ptr(self.device)
             _native.check(_native.lib().fluxb_int4_gemm(ctypes.byref(a)), "fluxb_int4_gemm")
         return out
 
@@ -223,7 +229,8 @@ class Int4GemmGrouped(_Int4Weights):
         if splits.numel() != self.E or splits.is_floating_point() or splits.dtype == torch.bool:
             raise ValueError(f"splits must hold one row count for each of {self.E} experts")
         if input.is_cuda:
-            splits = splits.reshape(-1).to(device=input.device, dtype=torch.int32, non_blocking=True).contiguous()
+            if splits.dtype != torch.int32 or splits.device != self.device or not splits.is_contiguous():
+                splits = splits.to(device=self.device, dtype=torch.int32, non_blocking=True).contiguous()
             return self._launch(input, None, splits, output_buf)
         y = output_buf if output_buf is not None else torch.zeros((input.shape[0], self.N), dtype=input.dtype)
         row = 0

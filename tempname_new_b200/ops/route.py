@@ -5,6 +5,7 @@ top-k of the framework there (``python/flux/testing/moe_utils.py``). The kernel 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -15,6 +16,7 @@ from .. import _native
 from ._dense import current_stream_ptr, device_guard, dtype_code
 
 _VP = ctypes.c_void_p
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS, MAX_TOPK, MAX_GROUPS = 512, 32, 32
 
@@ -92,34 +94,59 @@ def moe_route_torch(logits: torch.Tensor, topk: int, score_func: str = "softmax"
     return experts.to(torch.int32), (w * scale).float()
 
 
-def _args(logits, experts, weights, cfg, device) -> RouteArgs:
+@functools.lru_cache(maxsize=256)
+def _plan(E: int, dtype: torch.dtype, topk: int, score_func: str, num_groups: int, topk_groups: int, group_top: int,
+          renormalize: bool, scale: float) -> RouteArgs:
+    """The checked arguments that do not depend on the tensors; to be copied by each call."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {dtype}")
+    if score_func not in _SCORES:
+        raise ValueError(f"score_func must be one of {tuple(_SCORES)}, got {score_func!r}")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"between 1 and {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= num_groups <= MAX_GROUPS or E % num_groups:
+        raise ValueError(f"{E} experts do not divide over {num_groups} groups (at most {MAX_GROUPS})")
+    if not 1 <= topk_groups <= num_groups:
+        raise ValueError("topk_groups must be between 1 and num_groups")
+    if group_top not in (1, 2) or (num_groups > 1 and group_top > E // num_groups):
+        raise ValueError("group_top must be 1 or 2, and no more than the experts of a group")
+    if not 1 <= topk <= min(MAX_TOPK, E // num_groups * topk_groups):
+        raise ValueError(f"topk must be between 1 and {min(MAX_TOPK, E // num_groups * topk_groups)}, got {topk}")
+    if not 2.0 ** -126 <= abs(scale) < 2.0 ** 127:
+        raise ValueError("scale must be finite and not zero (in 32 bits)")
     a = RouteArgs()
-    a.logits, a.row_stride, a.dtype = logits.data_ptr(), logits.stride(0), dtype_code(logits.dtype)
+    a.num_experts, a.topk, a.num_groups = E, topk, num_groups
+    a.topk_groups, a.group_top = (topk_groups, group_top) if num_groups > 1 else (1, 1)
+    a.score, a.renormalize, a.scale, a.dtype = _SCORES[score_func], renormalize, scale, dtype_code(dtype)
+    return a
+
+
+def _args(plan, x, experts, weights, device) -> RouteArgs:
+    a = RouteArgs.from_buffer_copy(plan)
+    a.logits, a.row_stride, a.tokens = x.data_ptr(), x.stride(0), x.shape[0]
     a.experts, a.weights = experts.data_ptr(), weights.data_ptr()
-    a.tokens, a.num_experts = logits.shape
-    a.topk, a.score, bias, a.num_groups, a.topk_groups, a.group_top, a.renormalize, a.scale = cfg
-    if bias is not None:
-        a.bias = bias.data_ptr()
     a.stream = current_stream_ptr(device)
     return a
 
 
-def _forward(logits, cfg):
+def _forward(logits, bias, plan):
     x = logits if logits.stride(1) == 1 or logits.shape[1] == 1 else logits.contiguous()
-    device, shape = x.device, (x.shape[0], cfg[0])
+    device, shape = x.device, (x.shape[0], plan.topk)
     experts, weights = x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
     with device_guard(device):
-        a = _args(x, experts, weights, cfg, device)
+        a = _args(plan, x, experts, weights, device)
+        if bias is not None:
+            a.bias = bias.data_ptr()
         _native.check(_native.lib().fluxb_moe_route(ctypes.byref(a)), "fluxb_moe_route")
     return x, experts, weights
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, cfg):
-        x, experts, weights = _forward(logits, cfg)
+    def forward(ctx, logits, bias, plan):
+        x, experts, weights = _forward(logits, bias, plan)
         ctx.save_for_backward(x, experts, weights)
-        ctx.cfg = cfg
+        ctx.plan = plan
         ctx.mark_non_differentiable(experts)
         return experts, weights
 
@@ -130,10 +157,10 @@ class _Route(torch.autograd.Function):
         grad = grad.to(torch.float32).contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         with device_guard(x.device):
-            a = _args(x, experts, weights, ctx.cfg, x.device)
+            a = _args(ctx.plan, x, experts, weights, x.device)
             a.grad, a.dlogits = grad.data_ptr(), dx.data_ptr()
             _native.check(_native.lib().fluxb_moe_route_bwd(ctypes.byref(a)), "fluxb_moe_route_bwd")
-        return dx, None
+        return dx, None, None
 
 
 def moe_route(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -147,36 +174,19 @@ def moe_route(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias
     equal ones by their index. The weights are the chosen experts' scores, divided by their sum (``renormalize``), times
     ``scale``; they carry the gradient to the logits. An expert whose logit is -inf is chosen only when no other is left,
     with weight 0; NaN ranks lowest and shows in the weights."""
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError(f"logits must be [tokens, experts], got {tuple(logits.shape)}")
-    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    E = logits.shape[1]
-    topk, num_groups, topk_groups, group_top = int(topk), int(num_groups), int(topk_groups), int(group_top)
-    if score_func not in _SCORES:
-        raise ValueError(f"score_func must be one of {tuple(_SCORES)}, got {score_func!r}")
-    if E > MAX_EXPERTS:
-        raise ValueError(f"at most {MAX_EXPERTS} experts, got {E}")
-    if not 1 <= num_groups <= MAX_GROUPS or E % num_groups:
-        raise ValueError(f"{E} experts do not divide over {num_groups} groups (at most {MAX_GROUPS})")
-    if not 1 <= topk_groups <= num_groups:
-        raise ValueError("topk_groups must be between 1 and num_groups")
-    if group_top not in (1, 2) or (num_groups > 1 and group_top > E // num_groups):
-        raise ValueError("group_top must be 1 or 2, and no more than the experts of a group")
-    if not 1 <= topk <= min(MAX_TOPK, E // num_groups * topk_groups):
-        raise ValueError(f"topk must be between 1 and {min(MAX_TOPK, E // num_groups * topk_groups)}, got {topk}")
-    scale = float(scale)
-    if scale == 0.0 or not math.isfinite(ctypes.c_float(scale).value) or ctypes.c_float(scale).value == 0.0:
-        raise ValueError("scale must be finite and not zero")
+    shape = logits.shape
+    if len(shape) != 2:
+        raise ValueError(f"logits must be [tokens, experts], got {tuple(shape)}")
+    E = shape[1]
+    plan = _plan(E, logits.dtype, int(topk), score_func, int(num_groups), int(topk_groups), int(group_top), bool(renormalize),
+                 float(scale))
     if bias is not None:
         if bias.shape != (E,) or bias.dtype != torch.float32 or bias.device != logits.device:
             raise ValueError("bias must be float32 [experts] on the device of the logits")
         bias = bias.detach().contiguous()
-    if num_groups == 1:
-        topk_groups = group_top = 1
     if not logits.is_cuda:
-        return moe_route_torch(logits, topk, score_func, bias, num_groups, topk_groups, group_top, renormalize, scale)
-    cfg = (topk, _SCORES[score_func], bias, num_groups, topk_groups, group_top, bool(renormalize), scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _Route.apply(logits, cfg)
-    return _forward(logits, cfg)[1:]
+        return moe_route_torch(logits, plan.topk, score_func, bias, plan.num_groups, plan.topk_groups, plan.group_top,
+                               renormalize, plan.scale)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Route.apply(logits, bias, plan)
+    return _forward(logits, bias, plan)[1:]
