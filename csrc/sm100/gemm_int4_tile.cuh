@@ -46,7 +46,7 @@ struct Int4TileCfg {
   // The smallest tiles wait for weights, and what a CTA does once per block (waits, issue) would hold them up: two CTAs share
   // an SM. With TOK = 64, which needs the shared memory, two sets of warps unpack instead.
   static constexpr int CTAS = TOK_ == 32 ? 2 : 1;
-  static constexpr int SUM_WARPS = CTAS == 2 ? 4 : 8, SETS = SUM_WARPS / 4, UNPACK_SETS = TOK_ == 64 ? 2 : 1;
+  static constexpr int SUM_WARPS = CTAS == 2 ? 4 : 8, SETS = SUM_WARPS / 4, UNPACK_SETS = TOK_ <= 64 ? 2 : 1;
   static constexpr int UNPACK_WARP0 = SUM_WARPS, X_WARP = SUM_WARPS + 4 * UNPACK_SETS, MMA_WARP = X_WARP + 1,
                        W_WARP = X_WARP + 2, TABLE_WARP = X_WARP + 3;
   static constexpr int THREADS = 32 * (X_WARP + 4);
@@ -378,14 +378,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
       const uint32_t dphase = (Cfg::HALVES == 2 ? before / Cfg::A_BUFS : before / Cfg::RING) & 1u;
       if (!mbar_wait_all_warp(wc, MbarPhase{wfull(slot), wphase, kSiteSmemFull})) break;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        constexpr int GPH = G < 64 ? 64 / G : 1;             // groups of the half
-        uint32_t w[2][4], zz[GPH], a[2][16];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
-                       : "r"(wring + slot * Cfg::W_BYTES + (2 * i + u) * 512));
+      for (int i = 0; i < 4; ++i) {                          // row block i % 2 of the warp's two, 64 columns i / 2
+        constexpr int GPH = G < 64 ? 64 / G : 1;             // groups of 64 columns
+        const int u = i / 2;
+        uint32_t w[4], zz[GPH], a[16];
+        ptx::ld_shared_v4(wring + slot * Cfg::W_BYTES + (2 * (i % 2) + u) * 512, w);
 #pragma unroll
         for (int j = 0; j < GPH; ++j) {
           zz[j] = 0x08080808u;
@@ -393,41 +390,32 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
             asm volatile("ld.shared.u32 %0, [%1];" : "=r"(zz[j]) : "r"(zring + slot * Cfg::Z_BYTES + (u * 64 / G + j) * 128));
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {                        // the warp's two row blocks
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t z = zz[s * 16 / G % GPH];
-            const uint32_t z0 = i == 0 ? int4::magic_zero<Cfg::F16, 0>(z) : int4::magic_zero<Cfg::F16, 2>(z);
-            const uint32_t z1 = i == 0 ? int4::magic_zero<Cfg::F16, 1>(z) : int4::magic_zero<Cfg::F16, 3>(z);
-            int4::unpack<Cfg::F16>(w[i][s], z0, z1, a[i][4 * s], a[i][4 * s + 1], a[i][4 * s + 2], a[i][4 * s + 3]);
-          }
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t z = zz[s * 16 / G % GPH];
+          const uint32_t z0 = i % 2 == 0 ? int4::magic_zero<Cfg::F16, 0>(z) : int4::magic_zero<Cfg::F16, 2>(z);
+          const uint32_t z1 = i % 2 == 0 ? int4::magic_zero<Cfg::F16, 1>(z) : int4::magic_zero<Cfg::F16, 3>(z);
+          int4::unpack<Cfg::F16>(w[s], z0, z1, a[4 * s], a[4 * s + 1], a[4 * s + 2], a[4 * s + 3]);
         }
-        if (u == 0) {
-          if (pending) publish(last);
-          pending = false;
+        if (i == 0) {
+          // (the block that was here before has been multiplied)
           if (count >= Cfg::A_BUFS && !mbar_wait_all_warp(wc, MbarPhase{done, dphase, kSiteTmemEmpty})) {
             ok = false;
             break;
           }
           ptx::tc_fence_after();
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          ptx::tmem_st_16x256b_x4(
-              tmem + (static_cast<uint32_t>(q * 32 + i * 16) << 16) + Cfg::A_COL + buf * 64 + u * 32, a[i]);
+        ptx::tmem_st_16x256b_x4(
+            tmem + (static_cast<uint32_t>(q * 32 + (i % 2) * 16) << 16) + Cfg::A_COL + buf * 64 + u * 32, a);
       }
       if (!ok) break;
-      pending = true;
-      last = buf;
-      __syncwarp();
       if (lane == 0) ptx::mbar_arrive(wempty(slot));       // (the words have been read: they are in the stores)
+      publish(buf);
       slot += Cfg::UNPACK_SETS;
       if (slot >= Cfg::W_STAGES) {
         slot -= Cfg::W_STAGES;
         wphase ^= 1u;
       }
     }
-    if (pending) publish(last);
     drain();
     if (S > 1) ptx::cluster_sync();
     else __syncthreads();
