@@ -71,8 +71,8 @@ struct Int4TileCfg {
   static constexpr int SC_BYTES = GPS * 256;
   static constexpr int W_STAGES = TOK_ == 64 ? 6 : TOK_ == 256 ? 3 : 4;        // blocks of packed weights and zero points
   static constexpr int W_BYTES = 8192, Z_BYTES = GPS * 128;
-  static constexpr int EPI_PITCH = 36;                   // floats; a warp stages 16 rows of the output at a time
-  static constexpr int EPI_BYTES = SUM_WARPS * 16 * EPI_PITCH * 4;
+  static constexpr int EPI_PITCH = 40;                   // 16-bit values; a warp stages 16 rows of the output at a time
+  static constexpr int EPI_BYTES = SUM_WARPS * 16 * EPI_PITCH * 2;
   static constexpr int TAB_BYTES = (2 * (kInt4MaxExperts + 1) * 4 + 15) / 16 * 16;
   static constexpr int BAR_BYTES = 640;
   static constexpr int X_OFF = 0, SC_OFF = X_STAGES * XS_BYTES, W_OFF = SC_OFF + SC_SLOTS * SC_BYTES,
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
     const int set = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
     const int slot = (r / 64) * 64 + int4_scale_slot(r % 64);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    float* const stage = reinterpret_cast<float*>(sm + Cfg::EPI_OFF) + warp * (16 * Cfg::EPI_PITCH);
+    uint16_t* const stage = reinterpret_cast<uint16_t*>(sm + Cfg::EPI_OFF) + warp * (16 * Cfg::EPI_PITCH);
     const uint16_t* const scales = reinterpret_cast<const uint16_t*>(sm + Cfg::SC_OFF) + slot;
     uint32_t blocks = 0, blocks1 = 0;            // so far; with a second half
     bool ok = true;
@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
         continue;
       }
       // 16 rows of x by this warp's 32 rows of the weights, turned around in shared memory (nobody waits for other warps)
+      const float bias = p.bias != nullptr && it.n0 + r < p.N ? ptx::half_bits_to_float(p.bias[it.n0 + r], Cfg::F16) : 0.f;
 #pragma unroll
       for (int c0 = 0; c0 < CPT; c0 += 16) {
         const int m0 = c0 / CPD * NMMA + set * CPD + c0 % CPD;
@@ -304,18 +305,27 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
         if (live <= 0) break;
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
-          stage[c * Cfg::EPI_PITCH + lane] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2]));
-          stage[(c + 1) * Cfg::EPI_PITCH + lane] = __uint_as_float(static_cast<uint32_t>(acc[(c0 + c) / 2] >> 32));
+          const uint64_t two = acc[(c0 + c) / 2];
+          const uint32_t w = ptx::pack_half2(Cfg::F16, __uint_as_float(static_cast<uint32_t>(two)) + bias,
+                                             __uint_as_float(static_cast<uint32_t>(two >> 32)) + bias);
+          stage[c * Cfg::EPI_PITCH + lane] = static_cast<uint16_t>(w);
+          stage[(c + 1) * Cfg::EPI_PITCH + lane] = static_cast<uint16_t>(w >> 16);
         }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int m = i * 8 + lane / 4, n = it.n0 + quad * 32 + lane % 4 * 8;
           if (m < live && n < p.N) {
-            const float4 a = *reinterpret_cast<const float4*>(stage + m * Cfg::EPI_PITCH + lane % 4 * 8);
-            const float4 b = *reinterpret_cast<const float4*>(stage + m * Cfg::EPI_PITCH + lane % 4 * 8 + 4);
-            float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            store8(v, static_cast<int64_t>(it.row) + m0 + m, n);
+            const uint4 o = *reinterpret_cast<const uint4*>(stage + m * Cfg::EPI_PITCH + lane % 4 * 8);
+            uint16_t* const out = p.out + (static_cast<int64_t>(it.row) + m0 + m) * p.ldo + n;
+            if (tp.out_vec && n + 8 <= p.N) {
+              ptx::st_global_v4(out, o);
+            } else {
+              const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (n + k < p.N) out[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+            }
           }
         }
         __syncwarp();
