@@ -1,5 +1,5 @@
 // Host side of the products with 4-bit weights: layout of the weights, argument checks, choice of the kernel, launches.
-#include "int4_tile.h"
+#include "int4_launch.h"
 
 #include <atomic>
 
@@ -41,53 +41,6 @@ __global__ void int4_layout_scales_kernel(const fluxb_int4_layout_t a, int Np, i
     static_cast<uint16_t*>(a.scales_out)[to] = in ? static_cast<const uint16_t*>(a.scales)[from] : 0;
     if (a.zeros_out != nullptr) a.zeros_out[to] = in ? a.zeros[from] & 15 : 8;
   }
-}
-
-template <bool F16, bool SF16, int G, int NT>
-int launch_small(const Int4Params& p, cudaStream_t stream) {
-  using Cfg = Int4SmallCfg<G, NT>;
-  static bool configured[64] = {false};
-  int dev = 0;
-  FLUXB_CUDA_OK(cudaGetDevice(&dev));
-  if (dev >= 64 || !configured[dev]) {
-    FLUXB_CUDA_OK(cudaFuncSetAttribute(int4_small_kernel<F16, SF16, G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       Cfg::SMEM_BYTES));
-    if (dev < 64) configured[dev] = true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.tiles * p.splits_k, 1, 1);
-  cfg.blockDim = dim3(kInt4Warps * 32, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.splits_k;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.splits_k > 1 ? 1 : 0;
-  FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_small_kernel<F16, SF16, G, NT>, p));
-  FLUXB_CUDA_OK(cudaGetLastError());
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return kOk;
-}
-
-template <bool F16, bool SF16, int G>
-int launch_small(const Int4Params& p, int64_t rows, cudaStream_t stream) {
-  if (rows <= 8) return launch_small<F16, SF16, G, 1>(p, stream);
-  return launch_small<F16, SF16, G, 2>(p, stream);
-}
-
-template <bool F16, bool SF16>
-int launch_small(const Int4Params& p, int G, int64_t rows, cudaStream_t stream) {
-  if (G == 32) return launch_small<F16, SF16, 32>(p, rows, stream);
-  if (G == 64) return launch_small<F16, SF16, 64>(p, rows, stream);
-  return launch_small<F16, SF16, 128>(p, rows, stream);
-}
-
-template <bool F16>
-int launch_small(const Int4Params& p, int G, int64_t rows, cudaStream_t stream) {
-  return p.scale_f16 ? launch_small<F16, true>(p, G, rows, stream) : launch_small<F16, false>(p, G, rows, stream);
 }
 
 int round128(int v) { return (v + 127) / 128 * 128; }
@@ -159,12 +112,21 @@ extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
   const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;      // of an expert, on average
   const int steps = p.Kp / 128;
   if (a->splits == nullptr && rows <= 16) {
-    p.tiles = (a->N + 63) / 64;
+    // Rows of the weights per CTA, and CTAs that share K (a cluster costs 1 - 2 us to start):
+    //  * 64 where that fills the chip: 1 x 16384 x 4096 12.2 us, with 32 rows 13.3, on clusters of two 14.4;
+    //  * 32 where it does not: 1 x 4096 x 4096 5.1, with 64 rows and clusters of four 6.0; 16 x 4096 x 4096 7.2 and 7.8;
+    //  * 64 and clusters again for a long K: 16 x 4096 x 16384 17.7, with 32 rows 20.7, on clusters of two 21.6.
+    const int t64 = (a->N + 63) / 64, t32 = (a->N + 31) / 32;
+    const int rb = t64 > sms || steps > 64 ? 4 : 2;
+    p.tiles = rb == 4 ? t64 : t32;
+    const int room = rb == 4 ? 2 * sms : sms;
     int s = 1;
-    while (s < 4 && 2 * s * p.tiles <= 2 * sms && steps >= 16 * s) s *= 2;
+    while (s < 4 && 2 * s * p.tiles <= room && steps >= 16 * s) s *= 2;
     p.splits_k = s;
-    return a->dtype == FLUXB_FP16 ? launch_small<true>(p, G, rows, stream) : launch_small<false>(p, G, rows, stream);
+    return a->dtype == FLUXB_FP16 ? int4_small_f16(p, rb, G, stream) : int4_small_bf16(p, rb, G, stream);
   }
+  // Otherwise a tile of x as high as the rows (of an expert, on average): 45 x 5003 x 4128 15.7 us on tiles of 64, 17.5 on 32;
+  // 256 rows over 64 experts: 234 on 32, 216 on 64; 288 rows per expert 228 on 256, 241 on 128.
   Int4TileParams tp = {};
   p.tiles = p.Np / 128;
   const int tok = rows <= (a->splits ? 24 : 32) ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;

@@ -1,6 +1,6 @@
 #pragma once
 
-#include "int4_tile.h"
+#include "int4_launch.h"
 
 #include <atomic>
 

@@ -114,26 +114,28 @@ __device__ __forceinline__ float half_to_float(uint32_t bits16) {
 // steps before: no barriers, few registers, and 50 KB and more in flight per SM, which is what 6.5 TB/s take.
 // ----------------------------------------------------------------------------------------
 constexpr int kInt4Warps = 8;
-constexpr int kInt4Rows = 64;
 
-template <int G, int NT>
+template <int G, int NT, int RB_>
 struct Int4SmallCfg {
+  static constexpr int RB = RB_, ROWS = 16 * RB_;                    // row blocks and rows of the weights
   static constexpr int TOK = 8 * NT;
   static constexpr int GPS = G < 64 ? 64 / G : 1;                    // groups per step of 64 columns
   static constexpr int DEPTH = 2;                                    // steps in the ring
   static constexpr int CTAS = NT == 1 ? 3 : 2;                       // per SM
-  // one step of one warp: weights [4 row blocks][lane] 16 bytes, scales [GPS][lane] 16, x [NT][4][lane] 8, zeros [GPS][lane] 8
-  static constexpr int SC_OFF = 2048, X_OFF = SC_OFF + GPS * 512, Z_OFF = X_OFF + NT * 1024, STEP = Z_OFF + GPS * 256;
-  static constexpr int PITCH = kInt4Rows + 4;                        // floats per token of a staged tile
+  // one step of one warp: weights [RB][lane] 16 bytes, scales [GPS][lane] 4 RB, x [NT][4][lane] 8, zeros [GPS][lane] 2 RB
+  static constexpr int SC_OFF = RB * 512, X_OFF = SC_OFF + GPS * RB * 128, Z_OFF = X_OFF + NT * 1024,
+                       STEP = Z_OFF + GPS * RB * 64;
+  static constexpr int PITCH = ROWS + 4;                             // floats per token of a staged tile
   static constexpr int RING_BYTES = kInt4Warps * DEPTH * STEP, TILE_BYTES = (kInt4Warps + 1) * TOK * PITCH * 4;
   static constexpr int SMEM_BYTES = RING_BYTES > TILE_BYTES ? RING_BYTES : TILE_BYTES;
 };
 
-template <bool F16, bool SF16, int G, int NT>
-__global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
+template <bool F16, bool SF16, int G, int NT, int RB>
+__global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT, RB>::CTAS)
     int4_small_kernel(const __grid_constant__ Int4Params p) {
   using H = int4::Half<F16>;
-  using Cfg = Int4SmallCfg<G, NT>;
+  using Cfg = Int4SmallCfg<G, NT, RB>;
+  constexpr int ROWS = Cfg::ROWS;
   constexpr int TOK = Cfg::TOK, PITCH = Cfg::PITCH, GPS = Cfg::GPS, DEPTH = Cfg::DEPTH;
   constexpr int SPG = 4 / GPS;                                       // MMAs per group and step
   extern __shared__ __align__(16) float smem[];                      // the rings, then [warps + 1][TOK][PITCH]
@@ -145,8 +147,9 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
   const int units = p.Kp / 64;
   const int u0 = static_cast<int>(static_cast<int64_t>(units) * rank / S);
   const int u1 = static_cast<int>(static_cast<int64_t>(units) * (rank + 1) / S);
-  const uint4* const wbase = p.packed + static_cast<int64_t>(tile / 2) * (p.Kp / 128) * 512 + tile % 2 * 256 + lane;
-  const int scale_base = tile * 64 + g * 8;
+  const uint4* const wbase =
+      p.packed + static_cast<int64_t>(tile * ROWS / 128) * (p.Kp / 128) * 512 + tile * ROWS % 128 / 16 * 64 + lane;
+  const int scale_base = tile * ROWS / 64 * 64 + g * 8 + tile * ROWS % 64 / 8;      // (slot of the first row block)
   const uint32_t ring = ptx::smem_u32(smem) + warp * (DEPTH * Cfg::STEP);
 
   const uint16_t* const x0 = p.x + g * p.ldx + t * 4;
@@ -155,12 +158,12 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
     if (u < u1) {
       const uint4* const wu = wbase + static_cast<int64_t>(u >> 1) * 512 + (u & 1) * 32;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) ptx::cp_async_16(to + r * 512 + lane * 16, wu + r * 64, 16);
+      for (int r = 0; r < RB; ++r) ptx::cp_async_16(to + r * 512 + lane * 16, wu + r * 64, 16);
 #pragma unroll
       for (int j = 0; j < GPS; ++j) {
         const int64_t at = scale_base + static_cast<int64_t>(u * 64 / G + j) * p.Np;
-        ptx::cp_async_16(to + Cfg::SC_OFF + j * 512 + lane * 16, p.scales + at, 16);
-        if (p.zeros != nullptr) ptx::cp_async_8(to + Cfg::Z_OFF + j * 256 + lane * 8, p.zeros + at, 8);
+        ptx::cp_async<RB * 4>(to + Cfg::SC_OFF + (j * 32 + lane) * RB * 4, p.scales + at);
+        if (p.zeros != nullptr) ptx::cp_async<RB * 2>(to + Cfg::Z_OFF + (j * 32 + lane) * RB * 2, p.zeros + at);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -177,9 +180,9 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
     }
     ptx::cp_async_commit();
   };
-  float acc[4][NT][4];
+  float acc[RB][NT][4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -191,24 +194,25 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
   for (int u = u0 + warp; u < u1; u += kInt4Warps) {
     ptx::cp_async_wait<DEPTH - 1>();
     const uint32_t from = ring + slot * Cfg::STEP;
-    uint32_t w[4][4];
+    uint32_t w[RB][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ptx::ld_shared_v4(from + r * 512 + lane * 16, w[r]);
-    uint32_t sc[GPS][4], zp[GPS][2], xf[NT][4][2];
+    for (int r = 0; r < RB; ++r) ptx::ld_shared(from + r * 512 + lane * 16, w[r]);
+    uint32_t sc[GPS][RB], zp[GPS][RB / 2], xf[NT][4][2];
 #pragma unroll
     for (int j = 0; j < GPS; ++j) {
-      ptx::ld_shared_v4(from + Cfg::SC_OFF + j * 512 + lane * 16, sc[j]);
-      zp[j][0] = zp[j][1] = 0x08080808u;
-      if (p.zeros != nullptr) ptx::ld_shared_v2(from + Cfg::Z_OFF + j * 256 + lane * 8, zp[j]);
+      ptx::ld_shared(from + Cfg::SC_OFF + (j * 32 + lane) * RB * 4, sc[j]);
+#pragma unroll
+      for (int r = 0; r < RB / 2; ++r) zp[j][r] = 0x08080808u;
+      if (p.zeros != nullptr) ptx::ld_shared(from + Cfg::Z_OFF + (j * 32 + lane) * RB * 2, zp[j]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) ptx::ld_shared_v2(from + Cfg::X_OFF + (n * 4 + s) * 256 + lane * 8, xf[n][s]);
+      for (int s = 0; s < 4; ++s) ptx::ld_shared(from + Cfg::X_OFF + (n * 4 + s) * 256 + lane * 8, xf[n][s]);
     fetch(u + DEPTH * kInt4Warps, slot);
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < RB; ++r) {
 #pragma unroll
       for (int j = 0; j < GPS; ++j) {
         const uint32_t zz = zp[j][r / 2];
@@ -241,14 +245,14 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
   // the warps' sums: D fragment rows are weights (g, g + 8), columns are tokens (2 t, 2 t + 1)
   float* mine = smem + (warp + 1) * TOK * PITCH;
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mine[(n * 8 + 2 * t + (i & 1)) * PITCH + r * 16 + g + (i >> 1) * 8] = acc[r][n][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < TOK * kInt4Rows; i += kInt4Warps * 32) {
-    const int at = (i / kInt4Rows) * PITCH + i % kInt4Rows;
+  for (int i = threadIdx.x; i < TOK * ROWS; i += kInt4Warps * 32) {
+    const int at = (i / ROWS) * PITCH + i % ROWS;
     float v = 0.f;
 #pragma unroll
     for (int wv = 1; wv <= kInt4Warps; ++wv) v += smem[wv * TOK * PITCH + at];
@@ -256,10 +260,10 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
   }
   if (S > 1) ptx::cluster_sync();
   else __syncthreads();
-      for (int i = rank * kInt4Warps * 32 + threadIdx.x; i < rows * kInt4Rows; i += S * kInt4Warps * 32) {
-    const int m = i / kInt4Rows, n = tile * 64 + i % kInt4Rows;
+      for (int i = rank * kInt4Warps * 32 + threadIdx.x; i < rows * ROWS; i += S * kInt4Warps * 32) {
+    const int m = i / ROWS, n = tile * ROWS + i % ROWS;
     if (n >= p.N) continue;
-    const uint32_t at = ptx::smem_u32(smem + m * PITCH + i % kInt4Rows);
+    const uint32_t at = ptx::smem_u32(smem + m * PITCH + i % ROWS);
     float v = 0.f;
     if (S > 1) {
       for (int c = 0; c < S; ++c) {
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT>::CTAS)
         v += part;
       }
     } else {
-      v = smem[m * PITCH + i % kInt4Rows];
+      v = smem[m * PITCH + i % ROWS];
     }
     if (p.bias != nullptr) v += ptx::half_bits_to_float(p.bias[n], F16);
     p.out[m * p.ldo + n] = static_cast<uint16_t>(ptx::pack_half2(F16, v, 0.f));

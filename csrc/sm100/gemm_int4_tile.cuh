@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
         constexpr int GPH = G < 64 ? 64 / G : 1;             // groups of 64 columns
         const int u = i / 2;
         uint32_t w[4], zz[GPH], a[16];
-        ptx::ld_shared_v4(wring + slot * Cfg::W_BYTES + (2 * (i % 2) + u) * 512, w);
+        ptx::ld_shared(wring + slot * Cfg::W_BYTES + (2 * (i % 2) + u) * 512, w);
 #pragma unroll
         for (int j = 0; j < GPH; ++j) {
           zz[j] = 0x08080808u;

@@ -301,8 +301,12 @@ __device__ __forceinline__ void cp_async_8(uint32_t smem_dst, const void* gsrc, 
                "l"(reinterpret_cast<uint64_t>(gsrc)), "r"(src_size)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_4(uint32_t smem_dst, const void* gsrc) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(gsrc)) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t smem_dst, const void* gsrc) {
+  if constexpr (BYTES == 16) cp_async_16(smem_dst, gsrc, 16);
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(gsrc)), "n"(BYTES)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // wait until at most N of this thread's groups are in flight; what the others copied is visible to this thread
@@ -617,11 +621,14 @@ __device__ __forceinline__ ulonglong2 ld_shared_v2_b64(uint32_t saddr) {
   return v;
 }
 
-__device__ __forceinline__ void ld_shared_v4(uint32_t saddr, uint32_t (&v)[4]) {
+__device__ __forceinline__ void ld_shared(uint32_t saddr, uint32_t (&v)[4]) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(saddr));
 }
-__device__ __forceinline__ void ld_shared_v2(uint32_t saddr, uint32_t (&v)[2]) {
+__device__ __forceinline__ void ld_shared(uint32_t saddr, uint32_t (&v)[2]) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(saddr));
+}
+__device__ __forceinline__ void ld_shared(uint32_t saddr, uint32_t (&v)[1]) {
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(saddr));
 }
 
 // 16 bytes of shared memory of any CTA of the cluster (shared::cluster address, see mapa_u32)
