@@ -113,7 +113,8 @@ int fluxb_decode_work_items(int32_t num_seg, int32_t seg_first, int32_t m_tiles_
 uint64_t fluxb_launch_count(void);
 
 /* The last GEMM that the calling thread launched: which kernel the rules chose, and how (tests, profiles). */
-enum { FLUXB_KERNEL_NONE = 0, FLUXB_KERNEL_PERSISTENT = 1, FLUXB_KERNEL_SPLIT_K = 2, FLUXB_KERNEL_GROUPED = 3 };
+enum { FLUXB_KERNEL_NONE = 0, FLUXB_KERNEL_PERSISTENT = 1, FLUXB_KERNEL_SPLIT_K = 2, FLUXB_KERNEL_GROUPED = 3,
+       FLUXB_KERNEL_INT4_ROWS = 4, FLUXB_KERNEL_INT4_TILES = 5 /* 4-bit weights: few rows, and more */ };
 typedef struct {
   int32_t kernel, tile_m, tile_n;   /* rows and columns of a tile */
   int32_t cta_group;                /* CTAs that share a tile's MMAs: 1 or 2 */

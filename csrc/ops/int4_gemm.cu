@@ -2,6 +2,7 @@
 #include "int4_launch.h"
 
 #include <atomic>
+#include <cmath>
 
 namespace fluxb {
 extern std::atomic<uint64_t> g_launches;
@@ -44,6 +45,27 @@ __global__ void int4_layout_scales_kernel(const fluxb_int4_layout_t a, int Np, i
 }
 
 int round128(int v) { return (v + 127) / 128 * 128; }
+
+// What a product on the tile kernel takes in us: `ctas` tiles (times CTAs that share K) of 32 << i rows of x, `blocks` blocks of
+// 128 columns each, clusters of `splits`. Start, time per block and cost of a cluster as measured on 256 x 1024, 512 x 8192,
+// 32 .. 100 x 1024 / 4096 at K = 128 .. 8192 (blocks: K = 8192 less 4096); two CTAs on an SM take 1.5 times as long each.
+// What it decides, in us: 256 x 1024 x 1024 7.5 on tiles of 32 (64: 8.0, 128: 9.1, 256: 12.6, on clusters of two 12.8);
+// 100 x 1024 x 8192 9.4 on 32 and clusters of eight (128: 36.5, clusters of eight 13.5); 512 x 8192 x 4096 30.8 on 256 (128: 39.3,
+// 64: 56, 32: 69); groups of 64 make large tiles wait for more sums: 512 x 8192 x 4096 41, 50, 64, 79.
+double int4_tile_us(int i, int splits, int G, double ctas, int blocks, int sms) {
+  static const double start[4] = {4.8, 4.8, 5.6, 7.0};
+  static const double block[3][4] = {{0.70, 0.75, 1.09, 1.88}, {0.37, 0.43, 0.65, 1.02}, {0.33, 0.38, 0.50, 0.70}};
+  static const double cluster[4][4] = {{0.0, 1.4, 1.5, 2.5}, {0.0, 1.4, 2.0, 2.6}, {0.0, 1.8, 3.0, 4.4}, {0.0, 3.2, 5.0, 8.4}};
+  // clusters of 1, 2, 4, 8; those between are in the middle
+  const int j = splits >= 8 ? 3 : splits >= 4 ? 2 : splits >= 2 ? 1 : 0;
+  const double extra = splits == 3 || splits == 6 ? 0.5 * (cluster[i][j] + cluster[i][j + 1]) : cluster[i][j];
+  double one = block[G == 32 ? 0 : G == 64 ? 1 : 2][i], rounds = ctas / sms;
+  if (i == 0 && rounds > 1.0) {
+    one *= 1.5;
+    rounds /= 2.0;
+  }
+  return start[i] + extra + one * blocks * (rounds <= 1.0 ? 1.0 : ceil(rounds));
+}
 
 bool shape_ok(int experts, int N, int K, int group) {
   return experts >= 1 && experts <= 512 && N >= 1 && N <= (1 << 24) && K >= 32 && K <= (1 << 24) &&
@@ -109,9 +131,8 @@ extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
   if ((rc = device_sm_count(&sms))) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(a->stream);
   const int G = a->group < 128 ? a->group : 128;
-  const int64_t rows = a->splits ? (a->M + p.E - 1) / p.E : a->M;      // of an expert, on average
   const int steps = p.Kp / 128;
-  if (a->splits == nullptr && rows <= 16) {
+  if (a->splits == nullptr && a->M <= 16) {
     // Rows of the weights per CTA, and CTAs that share K (a cluster costs 1 - 2 us to start):
     //  * 64 where that fills the chip: 1 x 16384 x 4096 12.2 us, with 32 rows 13.3, on clusters of two 14.4;
     //  * 32 where it does not: 1 x 4096 x 4096 5.1, with 64 rows and clusters of four 6.0; 16 x 4096 x 4096 7.2 and 7.8;
@@ -125,16 +146,34 @@ extern "C" int fluxb_int4_gemm(const fluxb_int4_gemm_t* a) {
     p.splits_k = s;
     return a->dtype == FLUXB_FP16 ? int4_small_f16(p, rb, G, stream) : int4_small_bf16(p, rb, G, stream);
   }
-  // Otherwise a tile of x as high as the rows (of an expert, on average): 45 x 5003 x 4128 15.7 us on tiles of 64, 17.5 on 32;
-  // 256 rows over 64 experts: 234 on 32, 216 on 64; 288 rows per expert 228 on 256, 241 on 128.
   Int4TileParams tp = {};
   p.tiles = p.Np / 128;
-  const int tok = rows <= (a->splits ? 24 : 32) ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  int tok = 0;
+  double best = 1e30;
+  for (int i = 0; i < 4; ++i) {
+    const int t = 32 << i, resident = sms * (t == 32 ? 2 : 1);
+    // row tiles: at most, and about so many (an expert's last tile is half full on average)
+    const int64_t most = (a->M + t - 1) / t + (a->splits ? p.E : 0);
+    double about = static_cast<double>((a->M + t - 1) / t);
+    if (a->splits) {
+      const double each = static_cast<double>(a->M) / p.E;
+      about = each < 1.0 ? static_cast<double>(a->M) : p.E * (each < 0.5 * t ? 1.0 : each / t + 0.5);
+    }
+    if (most * p.tiles >= (1ll << 31)) continue;
+    for (int splits : {1, 2, 3, 4, 6, 8}) {
+      // (large clusters need that many free SMs in one part of the chip: half of the CTAs that fit have to do)
+      if (splits > 1 && (most * p.tiles * splits > (splits > 4 ? resident / 2 : resident) || steps < 2 * splits)) break;
+      const double us = int4_tile_us(i, splits, G, about * p.tiles * splits, (steps + splits - 1) / splits, sms);
+      if (us < best) {
+        best = us;
+        tok = t;
+        p.splits_k = splits;
+      }
+    }
+  }
+  FLUXB_REQUIRE(tok != 0, "4-bit product: too many tiles");
   const int64_t items = ((a->M + tok - 1) / tok + (a->splits ? p.E : 0)) * p.tiles;
-  FLUXB_REQUIRE(items < (1ll << 31), "4-bit product: too many tiles");
   const int resident = sms * (tok == 32 ? 2 : 1);
-  p.splits_k = 1;
-  while (p.splits_k < 8 && (p.splits_k + 1) * items <= resident && steps >= 2 * (p.splits_k + 1)) ++p.splits_k;
   tp.p = p;
   tp.out_vec = a->ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(a->out) & 15) == 0;
   tp.timeout_ns = 2000000000ull;

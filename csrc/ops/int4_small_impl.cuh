@@ -35,6 +35,7 @@ int launch_small(const Int4Params& p, cudaStream_t stream) {
   FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_small_kernel<F16, SF16, G, NT, RB>, p));
   FLUXB_CUDA_OK(cudaGetLastError());
   g_launches.fetch_add(1, std::memory_order_relaxed);
+  note_gemm({FLUXB_KERNEL_INT4_ROWS, Cfg::TOK, Cfg::ROWS, 1, p.splits_k, 0});
   return kOk;
 }
 

@@ -37,6 +37,7 @@ int launch_int4_tile(Int4TileParams& tp, int grid, cudaStream_t stream) {
   FLUXB_CUDA_OK(cudaLaunchKernelEx(&cfg, int4_tile_kernel<Cfg>, tp));
   FLUXB_CUDA_OK(cudaGetLastError());
   g_launches.fetch_add(1, std::memory_order_relaxed);
+  note_gemm({FLUXB_KERNEL_INT4_TILES, Cfg::TOK, 128, 1, tp.p.splits_k, 0});
   return kOk;
 }
 

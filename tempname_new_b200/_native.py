@@ -151,12 +151,12 @@ class GemmLaunch(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "tile_m", "tile_n", "cta_group", "splits", "cooperative")]
 
 
-_KERNELS = ("none", "persistent", "split_k", "grouped")
+_KERNELS = ("none", "persistent", "split_k", "grouped", "int4_rows", "int4_tiles")
 
 
 def last_gemm() -> dict:
-    """Which kernel the calling thread's last GEMM launch took, and how: ``kernel`` ("persistent", "split_k" or
-    "grouped"), ``tile_m``, ``tile_n``, ``cta_group``, ``splits``, ``cooperative``."""
+    """Which kernel the calling thread's last GEMM launch took, and how: ``kernel`` ("persistent", "split_k", "grouped",
+    "int4_rows" or "int4_tiles"), ``tile_m``, ``tile_n``, ``cta_group``, ``splits``, ``cooperative``."""
     rec = GemmLaunch()
     check(lib().fluxb_last_gemm(ctypes.byref(rec)), "fluxb_last_gemm")
     out = {name: int(getattr(rec, name)) for name, _ in rec._fields_}

@@ -326,6 +326,58 @@ def test_int4(dev, flux, m, n, k, group, dtype, scale_dtype):
         oracle.assert_within(y, ref, bound)
 
 
+# (m, n, k) -> the kernel, rows of x per tile and CTAs per tile that the rules choose on 148 SMs
+VARIANTS4 = [
+    (1, 16400, 256, "int4_rows", 8, 1), (7, 9400, 8448, "int4_rows", 8, 2), (8, 1000, 4096, "int4_rows", 8, 4),
+    (3, 600, 8192, "int4_rows", 8, 4), (9, 16300, 384, "int4_rows", 16, 1), (16, 520, 16384, "int4_rows", 16, 4),
+    (17, 300, 128, "int4_tiles", 32, 1), (40, 1000, 1024, "int4_tiles", 32, None), (100, 1000, 8192, "int4_tiles", 32, None),
+    (33, 5003, 4224, "int4_tiles", None, 3), (200, 700, 4096, "int4_tiles", 64, None),
+    (60, 16384, 1024, "int4_tiles", 64, 1), (57, 16001, 640, "int4_tiles", 64, 1), (64, 5000, 6144, "int4_tiles", None, None),
+    (120, 16384, 1024, "int4_tiles", 128, 1), (101, 15999, 1152, "int4_tiles", 128, 1),
+    (512, 8192, 1024, "int4_tiles", 256, 1), (433, 8100, 1152, "int4_tiles", 256, 1), (385, 8192, 1024, "int4_tiles", 256, 1),
+    (900, 2000, 4096, "int4_tiles", 256, None),
+]
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k,kernel,rows,splits", VARIANTS4)
+def test_int4_variants(dev, flux, m, n, k, kernel, rows, splits, group):
+    """Every kernel, tile and split with every group size, on integers whose sums are exact (as above)."""
+    g = _gen(dev, m + n)
+    q, s, z = _made4(dev, (), n, k, group, True, k)
+    s = (2.0 ** torch.randint(-3, 1, s.shape, device=dev, generator=g)).bfloat16()
+    x = torch.randint(-3, 4, (m, k), device=dev, generator=g).bfloat16()
+    bias = torch.randint(-8, 9, (n,), device=dev, generator=g).bfloat16()
+    op = flux.Int4Gemm(q, s, z)
+    y = op.forward(x, bias=bias)
+    took = flux._native.last_gemm()
+    assert took["kernel"] == kernel
+    if group == 128:
+        assert rows in (None, took["tile_m"]) and splits in (None, took["splits"]), took
+    ref = x.double() @ oracle.weights4(q, s, z, group).t() + bias.double()
+    assert torch.equal(y, ref.bfloat16())
+    op.check_status()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("splits,n,k", [([600, 0, 257, 300], 8192, 1024), ([128, 129, 127, 1, 0, 383], 4000, 1152),
+                                        ([3, 0, 40, 8], 16000, 640), ([0, 5, 0, 0], 300, 4096), ([70, 60, 64, 1], 8200, 1024)])
+def test_int4_grouped_variants(dev, flux, splits, n, k, group):
+    g = _gen(dev, n + k)
+    rows, E = sum(splits), len(splits)
+    q, s, z = _made4(dev, (E,), n, k, group, True, k)
+    s = (2.0 ** torch.randint(-3, 1, s.shape, device=dev, generator=g)).half()
+    x = torch.randint(-3, 4, (rows, k), device=dev, generator=g).half() / 32
+    op = flux.Int4GemmGrouped(q, s, z)
+    y = op.forward(x, torch.tensor(splits, device=dev, dtype=torch.int32))
+    row = 0
+    for e, count in enumerate(splits):
+        ref = x[row:row + count].double() @ oracle.weights4(q[e], s[e], z[e], group).t()
+        assert torch.equal(y[row:row + count], ref.half()), (e, flux._native.last_gemm())
+        row += count
+    op.check_status()
+
+
 def test_int4_outliers(dev, flux):
     """One huge activation next to small ones, a large mean: nothing cancels on the way."""
     q, s, z = _made4(dev, (), 200, 1024, 128, True, 4)
