@@ -5,9 +5,9 @@
 // through shared memory, whose bandwidth (128 bytes a cycle for writing and reading both) would bound the kernel at half the
 // speed at which memory delivers the packed weights. x tiles arrive by TMA as the B operand.
 // Every group's product lands in a fresh accumulator; eight warps multiply it with the group's scale (a thread owns one row
-// of the weights, so that is one number) and add it to their fp32 sums in registers. With TOK = 256 the accumulator is two
-// halves of 128 columns: the sums of one half are taken while the other is multiplied, and one unpacked weight serves 256
-// rows. Smaller TOK alternate two accumulators between groups.
+// of the weights, so that is one number) and add it to their fp32 sums in registers. With TOK = 256 the tile is two
+// halves of 128 columns that take turns at two or three accumulators, and one unpacked weight serves 256 rows. Smaller TOK have
+// two to four accumulators for consecutive groups.
 //
 //   warps 0 .. 7    sums: TMEM lanes 32 (warp % 4), the first or second half of the columns (warp / 4); epilogue
 //                   (TOK = 32: warps 0 .. 3)
@@ -52,21 +52,25 @@ struct Int4TileCfg {
   static constexpr int THREADS = 32 * (X_WARP + 4);
   static constexpr int CPD = NMMA / SETS;                // columns of an accumulator that a thread reads
   static constexpr int CPT = CPD * HALVES;               // columns that it sums
-  // TMEM: accumulators in the first half of the CTA's columns, blocks of weights in the second
-  static constexpr int TMEM_COLS = 512 / CTAS, A_COL = TMEM_COLS / 2, A_BUFS = A_COL / 64, D_BUFS = A_COL / NMMA;
+  // TMEM: accumulators in the first half of the CTA's columns, blocks of weights in the second; with TOK = 256 and small
+  // groups three accumulators and two blocks: an accumulator comes round after about 850 cycles, a group of 64 columns
+  // multiplies in 260 (9216 rows over 32 experts, groups of 64: 229 us with two, 217 with three; 2048 x 12288 x 4096, groups
+  // of 128: 166 and 169)
+  static constexpr int TMEM_COLS = 512 / CTAS, A_COL = TOK_ == 256 && G_ < 128 ? 384 : TMEM_COLS / 2,
+                       A_BUFS = (TMEM_COLS - A_COL) / 64, D_BUFS = A_COL / NMMA;
   // x arrives in blocks of 128 columns, with TOK = 256 in halves of a block (shared memory holds two and a half of them)
   static constexpr int XS_PER_BLOCK = TOK_ == 256 ? 2 : 1;
   static constexpr int XS_BYTES = TOK_ * 256 / XS_PER_BLOCK;
   static constexpr int X_STAGES = TOK_ == 256 ? 5 : TOK_ == 64 ? 8 : 4;
   // One commit per group or block hands its product over; the last one of a block also frees its weights and its x. The
-  // barriers are a ring of RING blocks. (TOK = 256: one barrier per half, and commits of their own for x and weights.)
+  // barriers are a ring of RING blocks. (TOK = 256: one per accumulator, and commits of their own for x and weights.)
   static constexpr int RING = TOK_ == 256 ? 1 : X_STAGES;
   // Groups that are handed over at once: those of a block where the accumulators hold two blocks, else one. (HALVES == 2:
   // one half of one group.) A wait that finds its phase complete still costs a warp about 110 cycles.
   static constexpr int GRAN = HALVES == 1 && D_BUFS >= 2 * GPS ? GPS : 1;
   static constexpr int HPB = GPS / GRAN;                 // hand-overs per block (and half)
-  static constexpr int UNITS = HALVES == 2 ? 2 : D_BUFS / GRAN;
-  static constexpr int D_BARS = TOK_ == 256 ? 2 : RING * HPB;
+  static constexpr int UNITS = D_BUFS / GRAN;
+  static constexpr int D_BARS = TOK_ == 256 ? UNITS : RING * HPB;
   static constexpr int SC_SLOTS = TOK_ == 256 ? 8 : RING + (D_BUFS + GPS - 1) / GPS;  // blocks of scales, see the x warp
   static constexpr int SC_BYTES = GPS * 256;
   static constexpr int W_STAGES = TOK_ == 64 ? 6 : TOK_ == 256 ? 3 : 4;        // blocks of packed weights and zero points
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     uint16_t* const stage = reinterpret_cast<uint16_t*>(sm + Cfg::EPI_OFF) + warp * (16 * Cfg::EPI_PITCH);
     const uint16_t* const scales = reinterpret_cast<const uint16_t*>(sm + Cfg::SC_OFF) + slot;
-    uint32_t blocks = 0, blocks1 = 0;            // so far; with a second half
+    uint32_t blocks = 0, turn = 0, lap = 0;
     bool ok = true;
     for (int item = first; item < items && ok; item += stride) {
       const Item it = item_of(item);
@@ -239,20 +243,19 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
 #pragma unroll
       for (int i = 0; i < CPT / 2; ++i) acc[i] = 0ull;
       const bool both = it.last - it.row > NMMA;           // (TOK = 256) the second half has rows
-      for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks, blocks1 += both) {
+      for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks) {
 #pragma unroll
         for (int j = 0; j < GPS; ++j) {
           float f = 0.f;
 #pragma unroll
           for (int h = 0; h < Cfg::HALVES; ++h) {
             if (h == 1 && !both) break;
-            // hand-overs so far (TOK = 256: of this half)
-            const uint32_t count = Cfg::HALVES == 2 ? (h == 0 ? blocks : blocks1) * GPS + j : blocks * HPB + j / GRAN;
-            const uint32_t unit = Cfg::HALVES == 2 ? static_cast<uint32_t>(h) : count % Cfg::UNITS;
+            const uint32_t count = blocks * HPB + j / GRAN;      // of hand-overs (TOK = 256: `turn` and `lap` tell)
+            const uint32_t unit = Cfg::HALVES == 2 ? turn : count % Cfg::UNITS;
             const uint32_t d = unit * GRAN + j % GRAN;
             if (j % GRAN == 0) {
-              const uint32_t full = Cfg::HALVES == 2 ? static_cast<uint32_t>(h) : count % Cfg::D_BARS;
-              const uint32_t phase = (Cfg::HALVES == 2 ? count : count / Cfg::D_BARS) & 1u;
+              const uint32_t full = Cfg::HALVES == 2 ? turn : count % Cfg::D_BARS;
+              const uint32_t phase = (Cfg::HALVES == 2 ? lap : count / Cfg::D_BARS) & 1u;
               if (!mbar_wait_all_warp(wc, MbarPhase{dfull(full), phase, kSiteTmemFull})) {
                 ok = false;
                 break;
@@ -279,6 +282,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
               for (int k = 0; k < W / 2; ++k)
                 acc[(h * CPD + c) / 2 + k] =
                     ptx::ffma2(ptx::pack_b32x2(v[2 * k], v[2 * k + 1]), ff, acc[(h * CPD + c) / 2 + k]);
+            }
+            if (Cfg::HALVES == 2 && ++turn == Cfg::UNITS) {
+              turn = 0;
+              ++lap;
             }
           }
           if (!ok) break;
@@ -562,7 +569,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
         }
       } else {
         // (stage: that of the block's first 64 columns)
-        uint32_t use[2] = {0, 0};                // of the two accumulators
+        uint32_t turn = 0, lap = 0;              // accumulator, and how often it has been used
         for (int item = first; item < items && ok; item += stride) {
           const Item it = item_of(item);
           // a tile that ends early is multiplied as far as it goes, in steps of 16 rows
@@ -584,8 +591,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 if (h == halves) break;
-                const MbarPhase room = {dempty(h), (use[h] & 1u) ^ 1u, kSiteTmemEmpty};
-                ++use[h];
+                const MbarPhase room = {dempty(turn), (lap & 1u) ^ 1u, kSiteTmemEmpty};
                 if (h == 0 && j == 0) ok = GPS == 1 ? mbar_wait_all_warp(wc, a, xa, xb, room) : mbar_wait_all_warp(wc, a, xa, room);
                 else ok = h == 0 && j * G == 64 ? mbar_wait_all_warp(wc, xb, room) : mbar_wait_all_warp(wc, room);
                 if (!ok) break;
@@ -595,10 +601,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
                   for (int s = j * SPG; s < (j + 1) * SPG; ++s) {
                     const uint32_t b_lo = (s < 4 ? x0 : x1) + h * (NMMA * 128 / 16) + 2u * (s % 4);
                     const uint32_t shape = h == 0 ? idesc0 : idesc1;
-                    if (s == j * SPG) ptx::umma_ts_f16<false>(tmem + h * NMMA, a_col + s * 8, b_lo, shape);
-                    else ptx::umma_ts_f16<true>(tmem + h * NMMA, a_col + s * 8, b_lo, shape);
+                    if (s == j * SPG) ptx::umma_ts_f16<false>(tmem + turn * NMMA, a_col + s * 8, b_lo, shape);
+                    else ptx::umma_ts_f16<true>(tmem + turn * NMMA, a_col + s * 8, b_lo, shape);
                   }
-                  ptx::umma_commit(dfull(h));
+                  ptx::umma_commit(dfull(turn));
                   if (h == halves - 1) {
                     if (j * G < 64 && (j + 1) * G >= 64) ptx::umma_commit(xempty(stage));
                     if (j == GPS - 1) {
@@ -608,6 +614,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
                   }
                 }
                 __syncwarp();
+                if (++turn == Cfg::UNITS) {
+                  turn = 0;
+                  ++lap;
+                }
               }
               if (!ok) break;
             }
