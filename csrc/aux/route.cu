@@ -520,6 +520,7 @@ int route(const fluxb_route_args_t* a, bool backward) {
   if (a->tokens == 0) return kOk;
   FLUXB_REQUIRE(a->logits && a->experts && a->weights, "null routing tensors");
   FLUXB_REQUIRE(!backward || (a->grad && a->dlogits), "null gradients");
+  FLUXB_REQUIRE(!backward || (reinterpret_cast<uintptr_t>(a->dlogits) & 15) == 0, "dlogits must be 16-byte aligned");
   FLUXB_REQUIRE(a->row_stride >= 0, "row stride");
   FLUXB_REQUIRE(a->scale != 0.f && a->scale - a->scale == 0.f, "scale must be finite and not zero");
   RouteParams p = {};

@@ -202,6 +202,9 @@ def test_native_argument_checks(lib_built):
     assert lib.fluxb_moe_route(ctypes.byref(a)) == 1
     a = R.RouteArgs(tokens=0, num_experts=64, topk=8, num_groups=8, topk_groups=1, group_top=1, scale=1.0)
     assert lib.fluxb_moe_route(ctypes.byref(a)) == 0
+    a = R.RouteArgs(tokens=1, num_experts=64, topk=8, num_groups=1, topk_groups=1, group_top=1, scale=1.0, logits=16, experts=16,
+                    weights=16, grad=16, dlogits=24)
+    assert lib.fluxb_moe_route_bwd(ctypes.byref(a)) == 1 and b"dlogits" in lib.fluxb_last_error()
     b = G.GatedArgs(rows=3, cols=4, act=3)
     assert lib.fluxb_gated_act(ctypes.byref(b)) == 1 and lib.fluxb_gated_act_bwd(ctypes.byref(b)) == 1
     c = I.Int4Layout(experts=1, N=8, K=48, group=32)
