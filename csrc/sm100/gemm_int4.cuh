@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, Int4SmallCfg<G, NT, RB>::CTAS
   }
   if (S > 1) ptx::cluster_sync();
   else __syncthreads();
-      for (int i = rank * kInt4Warps * 32 + threadIdx.x; i < rows * ROWS; i += S * kInt4Warps * 32) {
+  for (int i = rank * kInt4Warps * 32 + threadIdx.x; i < rows * ROWS; i += S * kInt4Warps * 32) {
     const int m = i / ROWS, n = tile * ROWS + i % ROWS;
     if (n >= p.N) continue;
     const uint32_t at = ptx::smem_u32(smem + m * PITCH + i % ROWS);

@@ -8,6 +8,7 @@ import os
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 from ..tuning import table as _table
@@ -55,6 +56,13 @@ def dtype_code(dt: torch.dtype) -> int:
     if code is None:
         raise TypeError(f"unsupported dtype {dt}")
     return code
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent."""
+    if getattr(forward_ad, "_current_level", 0) < 0:         # (outside dual_level there are none)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # (the stream handle without a Stream object around it: 0.2 us instead of 4)

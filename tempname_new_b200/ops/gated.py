@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native
-from ._dense import ACT, current_stream_ptr, device_guard, dtype_code
+from ._dense import ACT, current_stream_ptr, device_guard, dtype_code, has_tangent
 
 _VP = ctypes.c_void_p
 _GELU_A, _GELU_B = 2.0 * math.sqrt(2.0 / math.pi), 0.044715
@@ -123,7 +123,7 @@ def gated_act(gate: torch.Tensor, up: Optional[torch.Tensor] = None, act: str = 
     up weights leaves it. ``row_weight [rows]`` (float32) scales whole rows: the routing weight of each expert-sorted row.
     ``num_rows`` (one int32 or int64 on the device) is the number of rows in use, for buffers that are sized without asking
     the device; the rows behind it become zeros, in ``out`` they stay as they are. Gradients reach ``gate``, ``up`` and
-    ``row_weight``; ``out`` is for calls without them."""
+    ``row_weight``; ``out`` is for calls without them, and may be ``gate`` or ``up`` (or the gate's half of ``gate``)."""
     if gate.dim() != 2 or (up is not None and up.shape != gate.shape):
         raise ValueError("gate and up must be [rows, cols] of one shape, or gate [rows, 2 * cols] alone")
     if up is None and gate.shape[1] % 2:
@@ -143,12 +143,14 @@ def gated_act(gate: torch.Tensor, up: Optional[torch.Tensor] = None, act: str = 
         raise ValueError("num_rows must be one int32 or int64 on the device of gate")
     grads = torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)
                                          or (row_weight is not None and row_weight.requires_grad))
+    grads = grads or has_tangent(gate, up, row_weight)             # (a tangent is refused by the function below)
     if out is not None:
         if grads:
             raise ValueError("out cannot be used where gradients are recorded")
         if out.shape != (rows, cols) or out.dtype != gate.dtype or out.device != gate.device or (
-                cols > 1 and out.stride(1) != 1):
-            raise ValueError("out must be [rows, cols] of the type of gate, on its device, with contiguous rows")
+                cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+            raise ValueError("out must be [rows, cols] of the type of gate, on its device, with contiguous rows that do not "
+                             "overlap")
     if not gate.is_cuda:
         g, u = (gate, up) if up is not None else (gate[:, :cols], gate[:, cols:])
         y = gated_act_torch(g, u, act, row_weight, num_rows)

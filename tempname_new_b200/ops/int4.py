@@ -14,7 +14,7 @@ import torch
 
 from .. import _native
 from ..parallel.symm import FluxTimeoutError
-from ._dense import current_stream_ptr, device_guard, dtype_code
+from ._dense import current_stream_ptr, device_guard, dtype_code, has_tangent
 
 _VP = ctypes.c_void_p
 _HALF = (torch.bfloat16, torch.float16)
@@ -154,7 +154,7 @@ class _Int4Weights:
             raise FluxTimeoutError("product with 4-bit weights: a wait inside the kernel timed out")
 
     # ------------------------------------------------------------------------------
-    def _check_input(self, x, output_buf):
+    def _check_input(self, x, output_buf, bias=None):
         shape, dtype = x.shape, x.dtype
         if len(shape) != 2 or shape[1] != self.K:
             raise ValueError(f"input must be [rows, {self.K}], got {tuple(shape)}")
@@ -162,11 +162,14 @@ class _Int4Weights:
             raise TypeError(f"input must be bfloat16 or float16, got {dtype}")
         if x.device != self.device:
             raise ValueError(f"input is on {x.device}, the weights on {self.device}")
-        if x.requires_grad and torch.is_grad_enabled():
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)) \
+                or has_tangent(x, bias):
             raise RuntimeError("products with 4-bit weights have no backward; call them under torch.no_grad()")
         if output_buf is not None and (output_buf.shape != (shape[0], self.N) or output_buf.dtype != dtype
-                                       or output_buf.device != self.device or (self.N > 1 and output_buf.stride(1) != 1)):
-            raise ValueError("output_buf must be [rows, N] of the input's type, on its device, with contiguous rows")
+                                       or output_buf.device != self.device or (self.N > 1 and output_buf.stride(1) != 1)
+                                       or (shape[0] > 1 and output_buf.stride(0) < self.N)):
+            raise ValueError("output_buf must be [rows, N] of the input's type, on its device, with contiguous rows that do "
+                             "not overlap")
 
     def _launch(self, x, bias, splits, output_buf):
         rows = x.shape[0]
@@ -199,7 +202,7 @@ class Int4Gemm(_Int4Weights):
 
     def forward(self, input: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 output_buf: Optional[torch.Tensor] = None) -> torch.Tensor:
-        self._check_input(input, output_buf)
+        self._check_input(input, output_buf, bias)
         if bias is not None:
             if bias.numel() != self.N or bias.shape[-1] != self.N or bias.dtype != input.dtype \
                     or bias.device != input.device:

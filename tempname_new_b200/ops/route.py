@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native
-from ._dense import current_stream_ptr, device_guard, dtype_code
+from ._dense import current_stream_ptr, device_guard, dtype_code, has_tangent
 
 _VP = ctypes.c_void_p
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -187,6 +187,6 @@ def moe_route(logits: torch.Tensor, topk: int, score_func: str = "softmax", bias
     if not logits.is_cuda:
         return moe_route_torch(logits, plan.topk, score_func, bias, plan.num_groups, plan.topk_groups, plan.group_top,
                                renormalize, plan.scale)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if (logits.requires_grad and torch.is_grad_enabled()) or has_tangent(logits):   # (a tangent is refused there)
         return _Route.apply(logits, bias, plan)
     return _forward(logits, bias, plan)[1:]

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import expert_ops_oracle as oracle
 import tempname_new_b200 as flux
@@ -97,7 +98,8 @@ def test_gated_refusals():
         flux.gated_act(x, x.bfloat16())
     for bad in (dict(act="tanh"), dict(act=None), dict(row_weight=torch.ones(5)), dict(row_weight=torch.ones(4).bfloat16()),
                 dict(row_weight=torch.ones(4, 1)), dict(num_rows=torch.tensor([1, 2])), dict(num_rows=torch.tensor(1.0)),
-                dict(out=torch.empty(4, 16)), dict(out=torch.empty(4, 8).bfloat16()), dict(out=torch.empty(8, 4).t())):
+                dict(out=torch.empty(4, 16)), dict(out=torch.empty(4, 8).bfloat16()), dict(out=torch.empty(8, 4).t()),
+                dict(out=torch.empty(1, 8).expand(4, 8))):
         with pytest.raises(ValueError):
             flux.gated_act(x, **bad)
     with pytest.raises(ValueError):
@@ -176,10 +178,15 @@ def test_int4_refusals():
         op.forward(x.double())
     with pytest.raises(RuntimeError):
         op.forward(x.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        op.forward(x, bias=torch.zeros(8, requires_grad=True))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError):
+        op.forward(forward_ad.make_dual(x, torch.ones_like(x)))
     with torch.no_grad():
-        op.forward(x.clone().requires_grad_(True))
+        op.forward(x.clone().requires_grad_(True), bias=torch.zeros(8, requires_grad=True))
     for bad in (dict(bias=torch.zeros(7)), dict(bias=torch.zeros(8).bfloat16()), dict(output_buf=torch.empty(3, 7)),
-                dict(output_buf=torch.empty(8, 3).t()), dict(output_buf=torch.empty(3, 8).half())):
+                dict(output_buf=torch.empty(8, 3).t()), dict(output_buf=torch.empty(3, 8).half()),
+                dict(output_buf=torch.empty(1, 8).expand(3, 8))):
         with pytest.raises(ValueError):
             op.forward(x, **bad)
     many = flux.Int4GemmGrouped(q.unsqueeze(0), s.unsqueeze(0), z.unsqueeze(0))
@@ -217,6 +224,20 @@ def test_native_argument_checks(lib_built):
         assert lib.fluxb_int4_gemm(ctypes.byref(d)) == 1, bad
     for f in (lib.fluxb_moe_route, lib.fluxb_gated_act, lib.fluxb_int4_layout, lib.fluxb_int4_gemm):
         assert f(None) == 1
+
+
+def test_forward_mode_on_the_cpu():
+    """Tangents pass through the statements in PyTorch: here they match the gradient's product with the direction."""
+    g = torch.Generator().manual_seed(3)
+    x, v = torch.randn(5, 16, generator=g, dtype=torch.float32), torch.randn(5, 16, generator=g)
+    for f in (lambda t: flux.moe_route(t, 3)[1], lambda t: flux.gated_act(t, act="gelu")):
+        with forward_ad.dual_level():
+            tangent = forward_ad.unpack_dual(f(forward_ad.make_dual(x, v))).tangent
+        leaf = x.clone().requires_grad_(True)
+        y = f(leaf)
+        d = torch.randn(y.shape, generator=g)
+        grad, = torch.autograd.grad(y, leaf, d)
+        torch.testing.assert_close((tangent * d).sum(), (grad * v).sum(), rtol=1e-4, atol=1e-4)
 
 
 def test_example_with_int4_weights():

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import expert_ops_oracle as oracle
 
@@ -275,6 +276,37 @@ def test_gated_strides_streams_and_graphs(dev, flux):
         y = flux.gated_act(x, row_weight=weight, num_rows=num)
         d = torch.autograd.grad(y, (x, weight), dy)
         assert torch.equal(gy, y) and all(torch.equal(a, b) for a, b in zip(gd, d))
+
+
+def test_gated_in_place(dev, flux):
+    """The result may go where the gate, the up values or the gate's half of both were."""
+    x = torch.randn(33, 2 * 1000, device=dev, generator=_gen(dev, 10)).bfloat16()
+    for cols in (1000, 999, 64, 3):
+        both = x[:, :2 * cols]
+        want = flux.gated_act(both)
+        for place in range(3):
+            work = both.clone()
+            gate, up = work[:, :cols], work[:, cols:]
+            if place == 0:
+                got = flux.gated_act(work, out=gate)
+            else:
+                got = flux.gated_act(gate, up, out=gate if place == 1 else up)
+            assert torch.equal(got, want)
+            assert torch.equal(*((up, both[:, cols:]) if place < 2 else (gate, both[:, :cols])))
+
+
+def test_tangents_are_refused(dev, flux):
+    """Forward-mode derivatives have no rule on the device: an error, not a result without its tangent."""
+    x = torch.randn(4, 16, device=dev, generator=_gen(dev, 11))
+    q, s, _ = _made4(dev, (), 8, 128, 128, False, 1)
+    wide = torch.ones(4, 128, device=dev, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for f in (lambda: flux.moe_route(dual, 2), lambda: flux.gated_act(dual), lambda: flux.gated_act(x, dual),
+                  lambda: flux.Int4Gemm(q, s).forward(forward_ad.make_dual(wide, torch.ones_like(wide)))):
+            with pytest.raises(RuntimeError):
+                f()
+        assert flux.gated_act(x).shape == (4, 8) and flux.moe_route(x, 2)[0].shape == (4, 2)
 
 
 # ------------------------------------------------------------------------------------------ 4-bit products
