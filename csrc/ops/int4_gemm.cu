@@ -54,7 +54,7 @@ int round128(int v) { return (v + 127) / 128 * 128; }
 // 64: 56, 32: 69); groups of 64 make large tiles wait for more sums: 512 x 8192 x 4096 41, 50, 64, 79.
 double int4_tile_us(int i, int splits, int G, double ctas, int blocks, int sms) {
   static const double start[4] = {4.8, 4.8, 5.6, 7.0};
-  static const double block[3][4] = {{0.70, 0.75, 1.09, 1.88}, {0.37, 0.43, 0.65, 1.02}, {0.33, 0.38, 0.50, 0.70}};
+  static const double block[3][4] = {{0.70, 0.75, 1.09, 1.63}, {0.37, 0.43, 0.65, 1.02}, {0.33, 0.38, 0.50, 0.70}};
   static const double cluster[4][4] = {{0.0, 1.4, 1.5, 2.5}, {0.0, 1.4, 2.0, 2.6}, {0.0, 1.8, 3.0, 4.4}, {0.0, 3.2, 5.0, 8.4}};
   // clusters of 1, 2, 4, 8; those between are in the middle
   const int j = splits >= 8 ? 3 : splits >= 4 ? 2 : splits >= 2 ? 1 : 0;

@@ -376,10 +376,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
     const uint32_t zring = base + Cfg::Z_OFF + (q / 2) * 64 + (lane >> 2) * 8 + (q % 2) * 4;
     const bool zeros = p.zeros != nullptr;
     const uint32_t total = first < items ? static_cast<uint32_t>((items - 1 - first) / stride + 1) * (kb1 - kb0) : 0u;
-    // Half a block at a time (64 columns): its words are unpacked while the stores of the half before are on their way to
-    // TMEM, which are waited for (and, at the end of a block, published) just before the next ones are issued.
-    uint32_t last = 0;           // buffer whose stores are on their way
-    bool pending = false, ok = true;
+    // 16 rows by 64 columns at a time: unpacked while the stores of those before are on their way to TMEM; a block's stores are
+    // waited for, and published, at its end.
+    bool ok = true;
     auto publish = [&](uint32_t buf) {
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
@@ -570,28 +569,33 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
       } else {
         // (stage: that of the block's first 64 columns)
         uint32_t turn = 0, lap = 0;              // accumulator, and how often it has been used
+        // (lets the compiler know that all lanes have the same)
+        auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
         for (int item = first; item < items && ok; item += stride) {
           const Item it = item_of(item);
           // a tile that ends early is multiplied as far as it goes, in steps of 16 rows
           const int live = __shfl_sync(0xffffffffu, min(it.last - it.row, TOK), 0);
           const int halves = live > NMMA ? 2 : 1;
-          const uint32_t idesc0 = ptx::umma_idesc(kFmt, kFmt, 128, min((live + 15) & ~15, NMMA));
-          const uint32_t idesc1 = ptx::umma_idesc(kFmt, kFmt, 128, max(min((live + 15 - NMMA) & ~15, NMMA), 16));
+          const uint32_t idesc0 = uniform(ptx::umma_idesc(kFmt, kFmt, 128, min((live + 15) & ~15, NMMA)));
+          const uint32_t idesc1 = uniform(ptx::umma_idesc(kFmt, kFmt, 128, max(min((live + 15 - NMMA) & ~15, NMMA), 16)));
           for (int kb = kb0; kb < kb1 && ok; ++kb, ++blocks) {
             const uint32_t buf = blocks % Cfg::A_BUFS;
             const int stage1 = stage + 1 == Cfg::X_STAGES ? 0 : stage + 1;
             const uint32_t phase1 = stage1 == 0 ? phase ^ 1u : phase;
-            const uint32_t x0 = ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage * Cfg::XS_BYTES);
-            const uint32_t x1 = ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage1 * Cfg::XS_BYTES);
-            const uint32_t a_col = tmem + Cfg::A_COL + buf * 64;
+            const uint32_t x0 = uniform(ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage * Cfg::XS_BYTES));
+            const uint32_t x1 = uniform(ptx::umma_desc_k_sw128_lo(base + Cfg::X_OFF + stage1 * Cfg::XS_BYTES));
+            const uint32_t a_col = uniform(tmem + Cfg::A_COL + buf * 64);
             const MbarPhase a = {afull(buf), blocks / Cfg::A_BUFS & 1u, kSiteSmemFull};
             const MbarPhase xa = {xfull(stage), phase, kSiteSmemFull}, xb = {xfull(stage1), phase1, kSiteSmemFull};
-#pragma unroll
+            // (groups of 32: the hand-overs of a block in a row are more instructions than the first cache of them holds; as a
+            // loop 2048 x 12288 x 4096 takes 411 us instead of 474. Two groups of 64 in a row measured the same.)
+#pragma unroll(G == 32 ? 1 : GPS)
             for (int j = 0; j < GPS; ++j) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 if (h == halves) break;
                 const MbarPhase room = {dempty(turn), (lap & 1u) ^ 1u, kSiteTmemEmpty};
+                const uint32_t to = uniform(tmem + turn * NMMA);
                 if (h == 0 && j == 0) ok = GPS == 1 ? mbar_wait_all_warp(wc, a, xa, xb, room) : mbar_wait_all_warp(wc, a, xa, room);
                 else ok = h == 0 && j * G == 64 ? mbar_wait_all_warp(wc, xb, room) : mbar_wait_all_warp(wc, room);
                 if (!ok) break;
@@ -601,8 +605,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS) int4_tile_kernel(cons
                   for (int s = j * SPG; s < (j + 1) * SPG; ++s) {
                     const uint32_t b_lo = (s < 4 ? x0 : x1) + h * (NMMA * 128 / 16) + 2u * (s % 4);
                     const uint32_t shape = h == 0 ? idesc0 : idesc1;
-                    if (s == j * SPG) ptx::umma_ts_f16<false>(tmem + turn * NMMA, a_col + s * 8, b_lo, shape);
-                    else ptx::umma_ts_f16<true>(tmem + turn * NMMA, a_col + s * 8, b_lo, shape);
+                    if (s == j * SPG) ptx::umma_ts_f16<false>(to, a_col + s * 8, b_lo, shape);
+                    else ptx::umma_ts_f16<true>(to, a_col + s * 8, b_lo, shape);
                   }
                   ptx::umma_commit(dfull(turn));
                   if (h == halves - 1) {
