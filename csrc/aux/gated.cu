@@ -6,6 +6,12 @@
 // fixed order.
 //
 // Rows past a device-side count are left as they are, or zeroed in a buffer that the caller has just made.
+//
+// One pass over memory in the widest pieces that every tensor's rows allow, 32 to 256 threads per row so that each has one
+// piece: 32768 x 2048 bf16 with the row weights' gradient 186 us in two kernels, 5.8 TB/s over the eight values read or written
+// (88 % of a plain copy; the backward has to read gate and up again). Rows that start on any 2 bytes have only 2-byte pieces,
+// four of them in flight per thread: 5000 x 1001 fp16 13.7 us, 2.2 TB/s, bound by instruction issue (one at a time: 19.6 us).
+// 512 x 1536 takes 2.8 us, little more than an empty kernel.
 #include "../include/fluxb.h"
 #include "../runtime/host_common.h"
 #include "../sm100/ptx.cuh"

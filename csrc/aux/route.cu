@@ -20,6 +20,11 @@
 // Otherwise scores are computed in 32 bits with a bound on their error, and a token two of whose candidates (or groups) next to
 // each other in the order are closer than that is decided again in 64 bits, by the warp that found it (about 3 tokens in a
 // thousand with normal logits over 256 experts).
+//
+// Bound by instructions, not by memory (kernels alone, the L2 holding the logits): 64 tokens over 64 experts 2.8 us, little more
+// than an empty kernel; 8192 x 256, 8 of them from 4 of 8 groups, bias: 16.6 us (0.5 TB/s, 67 % of the issue slots), 4 of them for
+// the tail of warps that decide close tokens again (12.3 without one), where scores in 64 bits throughout took 37; 16384 x 120
+// bf16, 6 of them, with the gradient: 19.8 us in two kernels.
 #include "../include/fluxb.h"
 #include "../runtime/host_common.h"
 #include "../sm100/ptx.cuh"

@@ -112,6 +112,11 @@ __device__ __forceinline__ float half_to_float(uint32_t bits16) {
 // the `splits_k` CTAs of a cluster in distributed shared memory, always in the same order. Up to 8 * NT rows of x.
 // What a lane needs for a step it copies itself into a ring of its own in shared memory (cp.async) while it works on the
 // steps before: no barriers, few registers, and 50 KB and more in flight per SM, which is what 6.5 TB/s take.
+//
+// Measured, bf16, groups of 128 (L2 cold): 1 x 16384 x 4096 11.6 us, 3.0 TB/s, of which 4 are start, first loads and the last
+// sums; a longer K adds weights at 4.3 TB/s. 16 x 4096 x 16384 fp16, groups of 64, zero points: 17.8 us, 2.1 TB/s. Bound by
+// the ALU, which takes 7 of the 11 instructions of each 8 weights at half rate (issue slots 56 % busy, ALU 54 %, tensor pipe 14 %),
+// and by 256 tiles on 148 SMs.
 // ----------------------------------------------------------------------------------------
 constexpr int kInt4Warps = 8;
 
