@@ -63,6 +63,8 @@ def _args(gate, up, act, row_weight, num_rows, device) -> GatedArgs:
         a.up, a.up_stride = gate.data_ptr() + cols * gate.element_size(), gate.stride(0)
     else:
         a.up, a.up_stride = up.data_ptr(), up.stride(0)
+    if cols >= 1 << 31:
+        raise ValueError(f"rows of {cols} columns are not supported")
     a.rows, a.cols = rows, cols
     a.dtype, a.act = dtype_code(gate.dtype), ACT[act]
     if row_weight is not None:

@@ -18,7 +18,7 @@ from ._dense import current_stream_ptr, device_guard, dtype_code, has_tangent
 
 _VP = ctypes.c_void_p
 _HALF = (torch.bfloat16, torch.float16)
-MAX_EXPERTS = 512
+MAX_EXPERTS, MAX_SIDE = 512, 1 << 24
 
 
 class Int4Layout(ctypes.Structure):
@@ -109,6 +109,8 @@ class _Int4Weights:
         if any(t is not None and t.device != qweight.device for t in (scales, zeros)):
             raise ValueError("qweight, scales and zeros must share a device")
         self.N, self.K = qweight.shape[-2], 2 * qweight.shape[-1]
+        if self.N > MAX_SIDE or self.K > MAX_SIDE:
+            raise ValueError(f"weights of at most {MAX_SIDE} rows and columns, got {self.N} and {self.K}")
         if self.N < 1 or self.K % scales.shape[-1]:
             raise ValueError(f"{scales.shape[-1]} scales per row do not divide K = {self.K}")
         self.group = self.K // scales.shape[-1]

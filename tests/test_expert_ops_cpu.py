@@ -226,6 +226,17 @@ def test_native_argument_checks(lib_built):
         assert f(None) == 1
 
 
+def test_sizes_beyond_the_arguments():
+    """Sizes that 32-bit arguments would wrap are refused."""
+    from tempname_new_b200.ops import gated as G
+    side = 1 << 25
+    with pytest.raises(ValueError):
+        flux.Int4Gemm(torch.empty(side, 16, dtype=torch.uint8, device="meta"),
+                      torch.empty(side, 1, dtype=torch.bfloat16, device="meta"))
+    with pytest.raises(ValueError):
+        G._args(torch.empty(1, 1 << 33, device="meta"), None, "silu", None, None, torch.device("cpu"))
+
+
 def test_forward_mode_on_the_cpu():
     """Tangents pass through the statements in PyTorch: here they match the gradient's product with the direction."""
     g = torch.Generator().manual_seed(3)

@@ -481,6 +481,33 @@ def test_int4_grouped(dev, flux, splits, zeros):
         assert torch.equal(short[:rows - splits[7]], out[:rows - splits[7]]) and bool((short[rows:] == 0).all())
 
 
+def test_offsets_beyond_32_bits(dev, flux):
+    """Rows and experts whose elements lie more than 2^31 behind the first: as in a call of their own. Activations -1, 0, 1
+    and scales of a power of two make every sum exact, so that tiles of any shape agree to the bit."""
+    g = _gen(dev, 5)
+    x = torch.randint(-1, 2, (300_000, 8192), device=dev, generator=g, dtype=torch.int8).bfloat16()
+    q, s, _ = _made4(dev, (), 130, 8192, 128, False, 1)
+    op = flux.Int4Gemm(q, torch.full_like(s, 0.0625))
+    y = op.forward(x)
+    assert torch.equal(y[-70:], op.forward(x[-70:])) and torch.equal(y[262_100:262_200], op.forward(x[262_100:262_200]))
+    both = x.view(150_000, 16384)[-140_000:]
+    act = flux.gated_act(both)
+    for part in (slice(-9, None), slice(131_060, 131_080)):
+        assert torch.equal(act[part], flux.gated_act(both[part]))
+    del both, act, y
+    idx, w = flux.moe_route(x.view(-1, 512)[:, 100:356], 4, "sigmoid")
+    few = flux.moe_route(x.view(-1, 512)[-40:, 100:356], 4, "sigmoid")
+    assert torch.equal(idx[-40:], few[0]) and torch.equal(w[-40:], few[1])
+    x = x[:40]
+    q = torch.randint(0, 256, (70, 8192, 4096), device=dev, dtype=torch.uint8, generator=g)
+    s = torch.full((70, 8192, 64), 0.0625, device=dev, dtype=torch.bfloat16)
+    splits = torch.zeros(70, device=dev, dtype=torch.int32)
+    splits[0], splits[-2], splits[-1] = 3, 20, 17
+    y = flux.Int4GemmGrouped(q, s).forward(x, splits)
+    for e, rows in ((0, slice(0, 3)), (68, slice(3, 23)), (69, slice(23, 40))):
+        assert torch.equal(y[rows], flux.Int4Gemm(q[e], s[e]).forward(x[rows]))
+
+
 def test_int4_streams_and_graphs(dev, flux):
     q, s, z = _made4(dev, (4,), 256, 512, 128, False, 2)
     dense, grouped = flux.Int4Gemm(q[0], s[0]), flux.Int4GemmGrouped(q, s)
