@@ -540,6 +540,43 @@ def test_int4_streams_and_graphs(dev, flux):
             assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+def test_calls_from_several_threads(dev, flux):
+    """One op used by four threads at once, each with its own stream, sizes and outputs."""
+    import threading
+    q, s, z = _made4(dev, (6,), 200, 384, 64, True, 4)
+    dense, grouped = flux.Int4Gemm(q[0], s[0], z[0]), flux.Int4GemmGrouped(q, s, z)
+    g = _gen(dev, 4)
+    work = []
+    for m in (3, 20, 75, 310):
+        x = torch.randn(m, 384, device=dev, generator=g).bfloat16()
+        splits = torch.tensor([m // 3, 0, m // 4, 0, 1, m - m // 3 - m // 4 - 1], device=dev, dtype=torch.int32)
+
+        def calls(x=x, splits=splits):
+            leaf = x.clone().requires_grad_(True)
+            idx, w = flux.moe_route(leaf[:, :64], 8, "sigmoid")
+            d, = torch.autograd.grad(w.sum() + flux.gated_act(leaf).sum(), leaf)
+            return idx, w.detach(), d, dense.forward(x), grouped.forward(x, splits)
+        work.append((calls, calls()))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(calls, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = calls()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        wrong.append("result")
+        except Exception as e:  # noqa: BLE001
+            wrong.append(repr(e))
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
+
+
 def test_expert_layer_together(dev, flux):
     """Router, index build, both products with 4-bit weights, activation with the routing weights, sum over the chosen
     experts - as a layer runs them - against the same steps in 64 bits on the rounded values in between."""
