@@ -383,7 +383,7 @@ typedef struct {
   int32_t* experts;          /* [tokens, topk]: written by the forward, read by the backward */
   float* weights;            /* [tokens, topk]: written by the forward, read by the backward */
   const float* grad;         /* backward: gradient of the weights */
-  void* dlogits;             /* backward: [tokens, num_experts] in the type of the logits */
+  void* dlogits;             /* backward: [tokens, num_experts] in the type of the logits, 16-byte aligned */
   int64_t tokens, row_stride;
   int32_t num_experts;       /* at most 512 */
   int32_t topk;              /* at most 32 */

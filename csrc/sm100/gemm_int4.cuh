@@ -65,6 +65,12 @@ struct Half<true> {
     __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<uint32_t*>(&r);
   }
+  // a / 16 + b
+  static __device__ __forceinline__ uint32_t sixteenth(uint32_t a, uint32_t b) {
+    const __half2 f = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x2c00)));
+    __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), f, *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
   // d = a * b + c
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
                                              float c2, float c3) {
@@ -78,19 +84,29 @@ struct Half<true> {
 // The four pairs of 16-bit floats q - z of one word; z0, z1: magic + zero point of rows g and g + 8, in both halves.
 // (Written as one three-input operation, since the compiler splits an AND and an OR with two constants: 13 ALU instructions
 // per word instead of 7, and the ALU, at half rate, is what limits the unpacking.)
+// fp16 has ten bits of mantissa: a nibble at bit 4 makes 1024 + 16 q there, and one multiply-add q - z, exactly. That saves two
+// of the three shifts; bf16's seven bits leave no room for it.
 template <bool F16>
 __device__ __forceinline__ void unpack(uint32_t w, uint32_t z0, uint32_t z1, uint32_t& r0a, uint32_t& r0b, uint32_t& r8a,
                                        uint32_t& r8b) {
   using H = Half<F16>;
-  auto pick = [](uint32_t v) {
+  auto pick = [](uint32_t v, uint32_t mask) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(0x000f000fu), "r"(H::kMagic));   // (v & mask) | magic
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(mask), "r"(H::kMagic));          // (v & mask) | magic
     return r;
   };
-  r0a = H::sub(pick(w), z0);
-  r0b = H::sub(pick(w >> 4), z0);
-  r8a = H::sub(pick(w >> 8), z1);
-  r8b = H::sub(pick(w >> 12), z1);
+  if constexpr (F16) {
+    const uint32_t n0 = H::sub(0x63806380u, z0), n1 = H::sub(0x63806380u, z1);                    // 960 - (1024 + z)
+    r0a = H::sub(pick(w, 0x000f000fu), z0);
+    r0b = H::sixteenth(pick(w, 0x00f000f0u), n0);
+    r8a = H::sub(pick(w >> 8, 0x000f000fu), z1);
+    r8b = H::sixteenth(pick(w >> 8, 0x00f000f0u), n1);
+  } else {
+    r0a = H::sub(pick(w, 0x000f000fu), z0);
+    r0b = H::sub(pick(w >> 4, 0x000f000fu), z0);
+    r8a = H::sub(pick(w >> 8, 0x000f000fu), z1);
+    r8b = H::sub(pick(w >> 12, 0x000f000fu), z1);
+  }
 }
 
 // magic + zero point, in both halves; I: which byte of zz
