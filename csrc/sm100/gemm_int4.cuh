@@ -11,7 +11,7 @@
 // A lane's four k are neighbours (instead of the pairs 2t and 2t + 8 of the instruction's own numbering: the order of the
 // terms of a sum is free as long as both operands agree), so that it also reads its activations 8 bytes at a time.
 // (w >> 4 i) & 0x000f000f | magic is then a pair of 16-bit floats 128 + q (bf16) or 1024 + q (fp16), and one packed
-// subtraction of magic + z gives the pair q - z: 11 instructions for 8 weights.
+// subtraction of magic + z gives the pair q - z: 11 instructions for 8 weights (9 in fp16).
 //   scales [Kp / G][Np], zeros likewise: inside 64 rows the order is (row % 8, row / 16, row / 8 % 2), so that a lane reads
 //   the eight values of its rows in four row blocks with one load.
 // Rows and columns up to Np and Kp are zero weights (q = z) with zero scales.
@@ -123,16 +123,16 @@ __device__ __forceinline__ float half_to_float(uint32_t bits16) {
 }  // namespace int4
 
 // ----------------------------------------------------------------------------------------
-// Few rows. A CTA owns 64 rows of the weights, its eight warps take 64 columns of k in turn: every weight is read and
+// Few rows. A CTA owns 64 (or 32) rows of the weights, its eight warps take 64 columns of k in turn: every weight is read and
 // converted once, every activation goes to the one warp that needs it, and the warps' sums meet in shared memory, those of
 // the `splits_k` CTAs of a cluster in distributed shared memory, always in the same order. Up to 8 * NT rows of x.
 // What a lane needs for a step it copies itself into a ring of its own in shared memory (cp.async) while it works on the
 // steps before: no barriers, few registers, and 50 KB and more in flight per SM, which is what 6.5 TB/s take.
 //
 // Measured, bf16, groups of 128 (L2 cold): 1 x 16384 x 4096 11.6 us, 3.0 TB/s, of which 4 are start, first loads and the last
-// sums; a longer K adds weights at 4.3 TB/s. 16 x 4096 x 16384 fp16, groups of 64, zero points: 17.8 us, 2.1 TB/s. Bound by
-// the ALU, which takes 7 of the 11 instructions of each 8 weights at half rate (issue slots 56 % busy, ALU 54 %, tensor pipe 14 %),
-// and by 256 tiles on 148 SMs.
+// sums; a longer K adds weights at 4.3 TB/s. 16 x 4096 x 16384 fp16, groups of 64, zero points: 17.4 us, 2.2 TB/s. Bound by
+// the ALU, which takes 7 of the 11 instructions of each 8 weights (fp16: 5 of 9) at half rate - issue slots 56 % busy, ALU 54 %,
+// tensor pipe 14 % -, and by 256 tiles on 148 SMs.
 // ----------------------------------------------------------------------------------------
 constexpr int kInt4Warps = 8;
 
